@@ -20,6 +20,8 @@ LOC_LA, LOC_LT, LOC_LAV, LOC_LCV, LOC_LWC, LOC_LBC, LOC_LWE, LOC_LPE, LOC_SIZE =
     0, 16, 272, 368, 2416, 3440, 3472, 3568, 5616
 
 MAX_ENS = 4
+F32, BF16, F16 = 0, 1, 2        # element types of the row operators (elg_amd/logits.py)
+TOP_MAX_K, ROW_MAX_V, DRAFT_MAX = 256, 1 << 24, 1024
 MAX_LOCAL_SIZE = 63             # ELG_SLOT_MAX - 1 (csrc/elg_rollout.h): k nearest neighbours + the depot slot, one slot per lane
 ROWS_LOCAL_SIZE = 47            # ELG_SLOT_STRIDE - 1: what the matrix-core kernels and the saved training rows are built for
 _vp = C.c_void_p
@@ -105,7 +107,8 @@ EXPORTS = ["elg_version", "elg_last_error", "elg_aug8", "elg_dist_matrix", "elg_
            "elg_encoder_ws_floats", "elg_encoder_fwd", "elg_encoder_bwd_ws_floats", "elg_encoder_bwd",
            "elg_local_fold_fwd", "elg_local_fold_bwd", "elg_check_feasible", "elg_rollout_stats", "elg_decoder_bwd",
            "elg_decoder_bwd_ws_floats",
-           "elg_rollout_scratch_floats", "elg_rollout_last_kernel"]
+           "elg_rollout_scratch_floats", "elg_rollout_last_kernel",
+           "elg_top_logits", "elg_distill_ws_bytes", "elg_distill_loss_grad", "elg_verify_draft"]
 
 _lib = None
 
@@ -163,6 +166,11 @@ def lib() -> C.CDLL:
         L.elg_decoder_bwd_ws_floats.argtypes = [i, i64, i]
         L.elg_decoder_bwd_ws_floats.restype = i64
         L.elg_decoder_bwd.restype = C.c_int
+        L.elg_top_logits.argtypes = [f, i64, i, i64, i64, i, fl, f, f, f, f]
+        L.elg_distill_ws_bytes.argtypes = [i64, i64, i]
+        L.elg_distill_ws_bytes.restype = i64
+        L.elg_distill_loss_grad.argtypes = [f, i64, i, i64, i64, f, i, f, i, i, f, fl, f, f, i, fl, f, f, f, f, i64, f]
+        L.elg_verify_draft.argtypes = [f, i64, i64, f, i64, i64, i, f, i, i64, f, i64, f, i64, i, i64, f, f, f]
         L.elg_check_feasible.restype = C.c_int
         L.elg_rollout_stats.restype = C.c_int
         L.elg_local_fold_fwd.restype = C.c_int
@@ -172,7 +180,7 @@ def lib() -> C.CDLL:
         for n in ("elg_aug8", "elg_dist_matrix", "elg_nbr_tables", "elg_route_length", "elg_rollout_fwd",
                   "elg_rollout_bwd", "elg_glimpse_rows_bwd", "elg_glimpse_bwd_fused", "elg_gemm_f32",
                   "elg_pomo_loss", "elg_pomo_loss_grad", "elg_adam_step", "elg_local_bwd_rows",
-                  "elg_add_instnorm_fwd", "elg_add_instnorm_bwd"):
+                  "elg_add_instnorm_fwd", "elg_add_instnorm_bwd", "elg_top_logits", "elg_distill_loss_grad", "elg_verify_draft"):
             getattr(L, n).restype = C.c_int
         _lib = L
     return _lib

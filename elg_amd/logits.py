@@ -1,0 +1,249 @@
+"""Row operators over node logits and probabilities: a teacher's best logits, the loss that distils a policy from them, and the
+verification of drafted choices.  They work on rows as `engine.rollout_forward(..., dump="logits" / "probs")` returns them -- closed nodes
+-inf / 0 -- and on any other rows of 1 to 2^24 entries in f32, bf16 or f16.
+
+    values, idx, tail = top_logits(teacher_logits, 40, with_tail=True)          # once per teacher rollout; 8 bytes per kept logit
+    loss = distill_loss(student_logits, values, idx, tail=tail, temperature=2.0)   # differentiable in the student's logits
+    loss, grad = distill_loss_grad(student_logits, values, idx, tail=tail)      # loss and gradient from one read of the logits
+    tokens, accepted = verify_draft(target_probs, drafted, uniforms, draft_probs=draft_probs)
+
+Each is one call into libelg_hip.so (include/elg_hip.h) on the current stream, without a host synchronisation: capturable.  Inputs must
+live on the current device; rows may be strided views (the last dimension contiguous), others are copied."""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib as L
+from .engine import _need_cuda
+
+_TYPES = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
+
+
+def _stream() -> int:
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _p(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _type(t: torch.Tensor, what: str) -> int:
+    _need_cuda(t, what)
+    ty = _TYPES.get(t.dtype)
+    if ty is None:
+        raise ValueError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
+    return ty
+
+
+def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
+    """(..., V) as (R, V) with a contiguous last dimension; a view wherever the strides allow one."""
+    if t.dim() == 0 or not 1 <= t.shape[-1] <= L.ROW_MAX_V:
+        raise ValueError(f"{what} must have rows of 1 .. {L.ROW_MAX_V} entries, got shape {tuple(t.shape)}")
+    if t.dim() != 2:
+        t = t.reshape(t.shape[:-1].numel(), t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _temperature(t: float) -> float:
+    t = float(t)
+    if not 0.0 < t <= 3.0e38:
+        raise ValueError(f"the temperature must be positive and finite, got {t}")
+    return t
+
+
+def _per_row(t: Optional[torch.Tensor], lead, what: str) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    _need_cuda(t, what)
+    if t.shape != lead:
+        raise ValueError(f"{what} must hold one number per row: {tuple(lead)}, got {tuple(t.shape)}")
+    if t.dtype != torch.float32:
+        raise ValueError(f"{what} must be float32, got {t.dtype}")
+    return t.contiguous()
+
+
+def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0, with_tail: bool = False) -> Tuple[torch.Tensor, ...]:
+    """The k best logits of each row: (values (..., k) of the logits' type, idx (..., k) int32), best first; equal logits by the lower
+    index, NaN above +inf.  with_tail adds the probability under softmax(logits / temperature) of the nodes not among the k, (...) f32 --
+    what `distill_loss` takes as `tail`.  1 <= k <= min(V, 256).  A row with fewer than k open nodes is filled up with its closed ones
+    (-inf), lowest index first.  No gradient flows through (the teacher is a constant)."""
+    ty = _type(logits, "logits")
+    temperature = _temperature(temperature)
+    z = _rows(logits.detach(), "logits")
+    R, V = z.shape
+    k = int(k)
+    if not 1 <= k <= min(V, L.TOP_MAX_K):
+        raise ValueError(f"k must be 1 .. min(V, {L.TOP_MAX_K}), got k = {k} for rows of {V}")
+    lead = logits.shape[:-1]
+    values = torch.empty(*lead, k, dtype=z.dtype, device=z.device)
+    idx = torch.empty(*lead, k, dtype=torch.int32, device=z.device)
+    tail = torch.empty(lead, dtype=torch.float32, device=z.device) if with_tail else None
+    L.check(L.lib().elg_top_logits(_p(z), z.stride(0), ty, R, V, k, temperature, _p(values), _p(idx), _p(tail), _stream()),
+            "elg_top_logits")
+    return (values, idx, tail) if with_tail else (values, idx)
+
+
+class _Teacher:
+    """The checked arguments of a distillation call."""
+
+    def __init__(self, logits, values, idx, tail, temperature, weight):
+        self.type = _type(logits, "logits")
+        self.top_type = _type(values, "top_values")
+        _need_cuda(idx, "top_idx")
+        if idx.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"top_idx must be int32 or int64, got {idx.dtype}")
+        lead = logits.shape[:-1]
+        if values.shape != idx.shape or values.dim() == 0 or values.shape[:-1] != lead:
+            raise ValueError(f"top_values and top_idx must be {tuple(lead)} + (k,), got {tuple(values.shape)} and {tuple(idx.shape)}")
+        self.k = values.shape[-1]
+        if not 1 <= self.k <= L.TOP_MAX_K:
+            raise ValueError(f"1 .. {L.TOP_MAX_K} teacher entries a row, got {self.k}")
+        if torch.is_grad_enabled() and (values.requires_grad or (tail is not None and tail.requires_grad)
+                                        or (weight is not None and weight.requires_grad)):
+            raise ValueError("no gradient flows to the teacher's logits, the tail or the weights: detach them")
+        self.values, self.idx = values.contiguous(), idx.contiguous()
+        self.tail = _per_row(tail, lead, "tail")
+        self.weight = _per_row(weight, lead, "weight")
+        self.temperature = _temperature(temperature)
+        self.lead = lead
+
+    def call(self, z, *, cot=None, cot_stride=0, scale=1.0, rows=None, total=None, grad=None):
+        R, V = z.shape
+        ws, n = None, 0
+        lib = L.lib()
+        if total is not None:
+            n = lib.elg_distill_ws_bytes(R, V, self.type)
+            ws = torch.empty(n, dtype=torch.uint8, device=z.device)
+        L.check(lib.elg_distill_loss_grad(_p(z), z.stride(0), self.type, R, V, _p(self.values), self.top_type, _p(self.idx),
+                                          int(self.idx.dtype == torch.int64), self.k, _p(self.tail), self.temperature, _p(self.weight),
+                                          _p(cot), cot_stride, scale, _p(rows), _p(total), _p(grad), _p(ws), n, _stream()),
+                "elg_distill_loss_grad")
+
+
+def _scale(reduction: str, R: int) -> float:
+    if reduction not in ("none", "sum", "mean"):
+        raise ValueError(f"reduction must be 'none', 'sum' or 'mean', got {reduction!r}")
+    return 1.0 / R if reduction == "mean" and R > 0 else 1.0
+
+
+class _DistillLoss(torch.autograd.Function):
+    """Forward: the loss from one read of the logits.  Backward: the gradient from a second one, scaled by the cotangent on the device."""
+
+    @staticmethod
+    def forward(ctx, logits, teacher, reduction, *saved):
+        z = _rows(logits, "logits")
+        scale = _scale(reduction, z.shape[0])
+        ctx.teacher, ctx.scale, ctx.reduction = teacher, scale, reduction
+        ctx.save_for_backward(logits, *saved)        # the teacher's tensors too: writing to one before the backward is an error, not a wrong gradient
+        if reduction == "none":
+            loss = torch.empty(teacher.lead, dtype=torch.float32, device=z.device)
+            if z.shape[0]:
+                teacher.call(z, rows=loss)
+        else:
+            loss = torch.empty((), dtype=torch.float32, device=z.device)
+            teacher.call(z, total=loss, scale=scale)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gout):
+        logits = ctx.saved_tensors[0]
+        z = _rows(logits, "logits")
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        if z.shape[0]:
+            ctx.teacher.call(z, cot=gout.contiguous().float(), cot_stride=int(ctx.reduction == "none"), scale=ctx.scale, grad=grad)
+        return (grad, None, None) + (None,) * (len(ctx.saved_tensors) - 1)
+
+
+def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_idx: torch.Tensor, *, tail: Optional[torch.Tensor] = None,
+                 temperature: float = 1.0, weight: Optional[torch.Tensor] = None, reduction: str = "mean") -> torch.Tensor:
+    """Distillation of `logits` (..., V) from a teacher's best logits top_values (..., k) at nodes top_idx (..., k):
+
+        q = (1 - tail) softmax(top_values / T),   p = softmax(logits / T)
+        L = T^2 weight [ sum_j q_j (log q_j - log p_{i_j})  +  tail (log tail - log p(no entry's node)) ]
+
+    per row; reduction 'none' (...) f32, 'sum', or 'mean' over all rows.  tail (...) f32: the teacher's probability outside its entries
+    (`top_logits(with_tail=True)`), None: the entries hold everything.  weight (...) f32: 0 leaves a row out (it is not read) -- finished
+    trajectories.  Entries whose node lies outside [0, V) (-1: padding) or whose logit is -inf are absent; a node listed twice carries both
+    masses.  Rows without an open node or without an entry give loss 0 and gradient 0; a teacher probability on a closed node gives +inf.
+
+    The gradient reaches `logits` only, in their type, and can be taken once (no double backward); statistics and sums are f32, the sum over
+    the rows f64."""
+    t = _Teacher(logits, top_values, top_idx, tail, temperature, weight)
+    return _DistillLoss.apply(logits, t, reduction, *(x for x in (t.values, t.idx, t.tail, t.weight) if x is not None))
+
+
+def distill_loss_grad(logits: torch.Tensor, top_values: torch.Tensor, top_idx: torch.Tensor, *, tail: Optional[torch.Tensor] = None,
+                      temperature: float = 1.0, weight: Optional[torch.Tensor] = None,
+                      reduction: str = "mean") -> Tuple[torch.Tensor, torch.Tensor]:
+    """(loss, d loss / d logits) of `distill_loss` in one pass over the logits: for training loops that hand the gradient on themselves
+    (`logits.backward(grad)`), with the loss's own cotangent 1.  With reduction 'none' the gradient is that of the rows' sum."""
+    t = _Teacher(logits, top_values, top_idx, tail, temperature, weight)
+    z = _rows(logits.detach(), "logits")
+    scale = _scale(reduction, z.shape[0])
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if reduction == "none":
+        loss = torch.empty(t.lead, dtype=torch.float32, device=z.device)
+        if z.shape[0]:
+            t.call(z, rows=loss, grad=grad)
+    else:
+        loss = torch.empty((), dtype=torch.float32, device=z.device)
+        t.call(z, total=loss, grad=grad, scale=scale)
+    return loss, grad
+
+
+def _steps(t: torch.Tensor) -> torch.Tensor:
+    """(..., S, V) as (B, S, V) with a contiguous last dimension; a view wherever the strides allow one."""
+    if t.dim() != 3:
+        t = t.reshape(t.shape[:-2].numel(), *t.shape[-2:])
+    return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
+
+
+def verify_draft(target_probs: torch.Tensor, draft_tokens: torch.Tensor, uniforms: torch.Tensor, *,
+                 draft_probs: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Which drafted choices the target keeps, and what it answers instead of the first one it does not: speculative sampling from given
+    uniforms.  target_probs (..., G + 1, V): the target's probabilities at each draft and after the last; draft_tokens (..., G) int32 /
+    int64; uniforms (..., G + 1) f32 in [0, 1): one per acceptance test and, last, one for the draw; draft_probs (..., G, V) of the same
+    type, or None where the drafts were certain (greedy); lengths (...) int32: drafts of each sequence (clamped to 0 .. G), None: all G.
+
+    Returns tokens (..., G + 1) int32 -- the accepted drafts, the drawn choice, then -1 -- and accepted (...) int32.  A draft is kept while
+    u q(x) < p(x) (exact, in 64 bits); the draw is from max(p - q, 0) at the refused draft, from the target's next row if none was refused,
+    from the target's own row where nothing is left of it over the draft, and -1 where that row is empty.  A token outside [0, V) is refused."""
+    ty = _type(target_probs, "target_probs")
+    _need_cuda(draft_tokens, "draft_tokens")
+    _need_cuda(uniforms, "uniforms")
+    if draft_tokens.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"draft_tokens must be int32 or int64, got {draft_tokens.dtype}")
+    if uniforms.dtype != torch.float32:
+        raise ValueError(f"uniforms must be float32, got {uniforms.dtype}")
+    if draft_tokens.dim() == 0 or target_probs.dim() < 2:
+        raise ValueError("draft_tokens is (..., G), target_probs (..., G + 1, V)")
+    lead, G = draft_tokens.shape[:-1], draft_tokens.shape[-1]
+    V = target_probs.shape[-1]
+    if G > L.DRAFT_MAX or not 1 <= V <= L.ROW_MAX_V:
+        raise ValueError(f"up to {L.DRAFT_MAX} drafts over rows of 1 .. {L.ROW_MAX_V} probabilities, got {G} over {V}")
+    if target_probs.shape != (*lead, G + 1, V) or uniforms.shape != (*lead, G + 1):
+        raise ValueError(f"target_probs must be {(*lead, G + 1, V)} and uniforms {(*lead, G + 1)}, got {tuple(target_probs.shape)} "
+                         f"and {tuple(uniforms.shape)}")
+    p = _steps(target_probs.detach())
+    q = None
+    if draft_probs is not None and G > 0:
+        if draft_probs.shape != (*lead, G, V) or draft_probs.dtype != target_probs.dtype:
+            raise ValueError(f"draft_probs must be {(*lead, G, V)} of {target_probs.dtype}, got {tuple(draft_probs.shape)} of {draft_probs.dtype}")
+        _need_cuda(draft_probs, "draft_probs")
+        q = _steps(draft_probs.detach())
+    B = p.shape[0]
+    x, u = draft_tokens.contiguous(), uniforms.contiguous()
+    if lengths is not None:
+        _need_cuda(lengths, "lengths")
+        if lengths.shape != lead or lengths.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"lengths must be {tuple(lead)} int32 or int64, got {tuple(lengths.shape)} {lengths.dtype}")
+        lengths = lengths.to(torch.int32).contiguous()
+    tokens = torch.empty(*lead, G + 1, dtype=torch.int32, device=p.device)
+    accepted = torch.empty(lead, dtype=torch.int32, device=p.device)
+    L.check(L.lib().elg_verify_draft(_p(p), p.stride(0), p.stride(1), _p(q), q.stride(0) if q is not None else 0,
+                                     q.stride(1) if q is not None else 0, ty, _p(x), int(x.dtype == torch.int64), G, _p(u), G + 1,
+                                     _p(lengths), B, G, V, _p(tokens), _p(accepted), _stream()), "elg_verify_draft")
+    return tokens, accepted

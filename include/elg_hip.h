@@ -40,6 +40,13 @@ extern "C" {
 #define ELG_LOC_LWE 3472    /* [32][3]  We / sqrt(32)                                         */
 #define ELG_LOC_LPE 3568    /* [64][32] (be + PE[j]) / sqrt(32)                               */
 #define ELG_LOC_SIZE 5616
+/* element types of the row operators over node logits / probabilities (elg_top_logits and below) */
+#define ELG_F32 0
+#define ELG_BF16 1
+#define ELG_F16 2
+#define ELG_TOP_MAX_K 256          /* best logits kept of a row                                  */
+#define ELG_ROW_MAX_V (1 << 24)    /* logits of a row                                            */
+#define ELG_DRAFT_MAX 1024         /* drafted choices of a sequence                              */
 #define ELG_MAX_ENS 4       /* model_params['ensemble_size'] <= 4 local policies (models.py:296-298)   */
 
 const char* elg_version(void);
@@ -467,6 +474,45 @@ int elg_decoder_bwd(const elg_decoder_bwd_args* args, void* stream);
 /* Scratch of elg_decoder_bwd for N1 > 128: two (B,8,R,N1) buffers (glimpse weights / their cotangents) + the (B,R,128) query
  * cotangent rows; 0 for N1 <= 128. */
 int64_t elg_decoder_bwd_ws_floats(int32_t B, int64_t R, int32_t N1);
+
+/* ---------------------------------------------------------------------------------------------------------------------------
+ * Row operators over node logits / probabilities: what one policy leaves behind for another (its best logits), the loss that
+ * teaches the other on them, and the check of choices the other has drafted.  Rows as elg_rollout_fwd dumps them (full_probs:
+ * closed nodes -inf / 0), or anybody's rows of 1 .. ELG_ROW_MAX_V entries.  No 16-byte alignment is needed; strides are in
+ * elements.  `type`: ELG_F32 / ELG_BF16 / ELG_F16.  Nothing is kept between calls; workspaces are the call's own.
+ * ------------------------------------------------------------------------------------------------------------------------- */
+
+/* The k best logits of each row z[r z_stride + n], n < V: values (R,k) of the same type, idx (R,k), best first.  Equal logits: the
+ * lower index first; NaN ranks above +inf; -0 equals +0.  tail (R) or NULL: the probability, under softmax(z / temperature), of the
+ * nodes that are not among the k (0 for a row without an open node).  1 <= k <= min(V, ELG_TOP_MAX_K). */
+int elg_top_logits(const void* z, int64_t z_stride, int type, int64_t R, int64_t V, int k, float temperature, void* values,
+                   int32_t* idx, float* tail, void* stream);
+
+/* Distillation from a teacher's best logits.  top_values (R,k) of top_type at nodes top_idx (R,k) (int32, or int64 with idx_wide);
+ * an entry whose node lies outside [0, V) is absent.  q_j = (1 - tail_r) softmax_j(top_values / temperature), p = softmax(z / temperature):
+ *   L_r = temperature^2 weight_r [ sum_j q_j (log q_j - log p_(i_j)) + tail_r (log tail_r - log sum_(n no entry) p_n) ]
+ * tail (R) in [0, 1] or NULL (0), weight (R) or NULL (1).  A row of weight 0 is not read; it, a row without an open node and a row
+ * without an entry above -inf have loss 0 and gradient 0.  A teacher probability on a node the student has closed makes the loss +inf.
+ *   loss_rows (R) or NULL  = scale L_r
+ *   loss_total (1) or NULL = scale sum_r L_r, added in 64 bits in an order of its own fixed by R (needs ws)
+ *   grad (R,V) packed, of `type`, or NULL = scale cot_r dL_r/dz; cot: NULL (1), one number (cot_stride 0) or one per row (1)
+ * ws: elg_distill_ws_bytes() bytes, 8-byte aligned. */
+int64_t elg_distill_ws_bytes(int64_t R, int64_t V, int type);
+int elg_distill_loss_grad(const void* z, int64_t z_stride, int type, int64_t R, int64_t V, const void* top_values, int top_type,
+                          const void* top_idx, int idx_wide, int k, const float* tail, float temperature, const float* weight,
+                          const float* cot, int cot_stride, float scale, float* loss_rows, float* loss_total, void* grad, void* ws,
+                          int64_t ws_bytes, void* stream);
+
+/* Verification of drafted choices.  target rows p(b, i) at target + b target_bstride + i target_sstride, i <= G; draft rows q(b, i),
+ * i < G, or NULL (every draft was certain: q = 1 on it); tokens (B,G) int32 (int64 with tokens_wide); uniforms (B,G+1) in [0, 1);
+ * lengths (B) or NULL (G): drafts of each sequence.  Draft i is accepted while uniforms(b,i) q(x_i) < p(x_i); a token outside
+ * [0, V) is refused.  accepted (B) = the drafts in front of the first refusal; out_tokens (B,G+1) = these, then the first n with
+ * cumsum(r)_n > uniforms(b,G) sum(r), then -1; r = max(p - q, 0) at the refused draft, p where that is all zero or nothing was
+ * refused, and -1 is drawn where p is zero too.  Rows need not sum to 1; entries that are not positive count as 0. */
+int elg_verify_draft(const void* target, int64_t target_bstride, int64_t target_sstride, const void* draft, int64_t draft_bstride,
+                     int64_t draft_sstride, int type, const void* tokens, int tokens_wide, int64_t tokens_stride, const float* uniforms,
+                     int64_t uniforms_stride, const int32_t* lengths, int64_t B, int G, int64_t V, int32_t* out_tokens,
+                     int32_t* accepted, void* stream);
 
 #ifdef __cplusplus
 }
