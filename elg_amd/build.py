@@ -15,8 +15,10 @@ LIB = os.path.join(HERE, "libelg_hip.so")
 SOURCES = ["elg_fwd.hip", "elg_fwd_coop.hip", "elg_bwd.hip", "elg_gemm.hip", "elg_train.hip", "elg_local.hip", "elg_encoder.hip", "elg_enc.hip", "elg_enc_fused.hip", "elg_fold.hip", "elg_dbwd.hip",
            "elg_topk.hip", "elg_distill.hip", "elg_verify.hip"]
 HEADERS = ["elg_common.h", "elg_rollout.h", "elg_coop.h", "elg_bwd_internal.h", "elg_bf16.h", "elg_enc_internal.h", "elg_logits.h", os.path.join("..", "..", "include", "elg_hip.h")]
+# -packed-fp32-ops: hipcc otherwise forms packed f32 instructions from ordinary float code, some of whose forms are unreliable on this part
+# (the host pass does not know the feature and says so: harmless)
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-fast-math",
-         "-Wno-unused-value"]
+         "-Wno-unused-value", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc() -> str:

@@ -35,6 +35,9 @@ struct DistillArgs {
     long long g_stride;                   // bytes
 };
 
+constexpr float TINY_MASS = 1e-36f;       // a (log a - log p_rest) below this is nothing in f32
+__device__ __forceinline__ float ln(float x) { return __builtin_amdgcn_logf(x) * 0.6931471805599453f; }
+
 constexpr int SEG = 65536;                // window positions whose membership bits are held at a time
 
 // One workgroup per row, T >= ELG_TOP_MAX_K threads: thread j < k holds entry j.  C > 0: the row stays in registers, C chunks a thread;
@@ -209,6 +212,193 @@ __global__ __launch_bounds__(T) void distill_row_kernel(const DistillArgs A) {
     if (A.part && tid == 0) A.part[blockIdx.x] = lacc;
 }
 
+// Short rows, G lanes per row (16: four rows to a wave; 64: one).  Lane l holds the nodes n = i G + l, i < NE, and the entries
+// j = e G + l, e < KE, in registers; a row is read and written in runs of G elements, whatever its alignment.  The row's teacher masses are
+// spread over a row of LDS, one float per node, where the lane that owns the node picks them up: -0 marks a node of no entry, and
+// -0 + q = q exactly.  Waves never wait for each other.
+template <int G> __device__ __forceinline__ float gsum(float v) { return G == 16 ? row16_sum(v) : wave_sum(v); }
+template <int G> __device__ __forceinline__ float gmax(float v) { return G == 16 ? row16_max(v) : wave_max(v); }
+
+template <int DT, int G, int NE, int KE, bool TAIL>
+__global__ __launch_bounds__(256) void distill_small_kernel(const DistillArgs A) {
+    // a row of LDS is padded so that the rows of a wave's four groups start 16 banks apart
+    constexpr int RW = 64 / G, P = G * NE + (G == 16 ? 16 : 0);
+    __shared__ float qs_all[4 * RW * P];
+    __shared__ double dred[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane / G, l = lane % G, V = A.V, k = A.k;
+    float* qs = qs_all + (wave * RW + g) * P;
+    const bool plain_entries = A.tv_type == ELG_F32 && !A.ti_wide;
+    const float inv_tau = 1.f / A.tau;
+    double lacc = 0.0;
+    for (long long r0 = ((long long)blockIdx.x * 4 + wave) * RW; r0 < A.R; r0 += (long long)gridDim.x * 4 * RW) {
+        const long long r = r0 + g;
+        const bool valid = r < A.R;
+        const float w = !valid ? 0.f : A.weight ? A.weight[r] : 1.f;
+        const bool on = w != 0.f;
+        const elem_t<DT>* row = reinterpret_cast<const elem_t<DT>*>(A.z + (valid ? r : 0) * A.z_stride);
+        // ---- entries and nodes
+        const int kk = on ? k : 0, vv = on ? V : 0;
+        int ei[KE];
+        float et[KE], zi[KE];
+        if (plain_entries) {
+            const int* ti = reinterpret_cast<const int*>(A.ti) + r * k;
+            const float* tv = reinterpret_cast<const float*>(A.tv) + r * k;
+#pragma unroll
+            for (int e = 0; e < KE; ++e) {
+                const int j = e * G + l;
+                ei[e] = j < kk ? ti[j] : -1;
+                et[e] = j < kk ? tv[j] : ELG_NEG_INF;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < KE; ++e) {
+                const int j = e * G + l;
+                ei[e] = -1;
+                et[e] = ELG_NEG_INF;
+                if (j < kk) {
+                    const long long i = index_any(A.ti, r * k + j, A.ti_wide);
+                    ei[e] = i >= 0 && i < V ? (int)i : -1;
+                    et[e] = elem_any(A.tv, r * k + j, A.tv_type);
+                }
+            }
+        }
+        float v[NE];
+#pragma unroll
+        for (int i = 0; i < NE; ++i) v[i] = i * G + l < vv ? (float)row[i * G + l] : ELG_NEG_INF;
+#pragma unroll
+        for (int e = 0; e < KE; ++e) {
+            const bool ok = (unsigned)ei[e] < (unsigned)V;
+            ei[e] = ok ? ei[e] : -1;
+            et[e] = ok ? et[e] : ELG_NEG_INF;
+            zi[e] = ok ? (float)row[ei[e]] : ELG_NEG_INF;
+        }
+        float a = TAIL && on ? A.tail[r] : 0.f;
+        a = a > 1.f ? 1.f : a < 0.f ? 0.f : a;
+        // ---- the teacher's masses
+        float tm = et[0];
+#pragma unroll
+        for (int e = 1; e < KE; ++e) tm = fmaxf(tm, et[e]);
+        tm = gmax<G>(tm);
+        tm = tm > ELG_NEG_INF ? tm : 0.f;
+        float q[KE], st = 0.f;
+#pragma unroll
+        for (int e = 0; e < KE; ++e) {
+            q[e] = ei[e] >= 0 ? ex2((et[e] - tm) * A.c2) : 0.f;
+            st += q[e];
+        }
+        st = gsum<G>(st);
+        const float qscale = st <= 0.f ? 0.f : (1.f - a) * __builtin_amdgcn_rcpf(st);
+#pragma unroll
+        for (int e = 0; e < KE; ++e) q[e] *= qscale;
+        auto clear = [&]() {
+            wave_lds_fence();
+#pragma unroll
+            for (int i = 0; i < NE; ++i) qs[i * G + l] = -0.f;
+            wave_lds_fence();
+        };
+        clear();
+        bool twice = false;
+#pragma unroll
+        for (int e = 0; e < KE; ++e)
+            if (ei[e] >= 0) {
+                const float old = __hip_atomic_fetch_add(qs + ei[e], q[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                twice = twice || f2i(old) != (int)0x80000000;
+            }
+        if (__any(twice)) {               // some node is listed twice: add its masses again, in entry order, so that the bits are the same in every run
+            clear();
+#pragma unroll
+            for (int e = 0; e < KE; ++e)
+#pragma unroll 1
+                for (int j = 0; j < G; ++j) {
+                    if (j == l && ei[e] >= 0) qs[ei[e]] += q[e];
+                    wave_lds_fence();
+                }
+        }
+        wave_lds_fence();
+        float qv[NE];
+#pragma unroll
+        for (int i = 0; i < NE; ++i) qv[i] = qs[i * G + l];
+        // ---- the student's softmax; v becomes e^(z - its part's maximum)
+        float m, S, f_top = 1.f, f_rest = 0.f, s_rest = 0.f, m_rest = 0.f;
+        if (TAIL) {
+            float mt = ELG_NEG_INF, mr = ELG_NEG_INF;
+#pragma unroll
+            for (int i = 0; i < NE; ++i) {
+                const bool top = f2i(qv[i]) >= 0;
+                mt = fmaxf(mt, top ? v[i] : ELG_NEG_INF);
+                mr = fmaxf(mr, top ? ELG_NEG_INF : v[i]);
+            }
+            mt = gmax<G>(mt);
+            mr = gmax<G>(mr);
+            m = fmaxf(mt, mr);
+            const float m_top = mt > ELG_NEG_INF ? mt : 0.f;
+            m_rest = mr > ELG_NEG_INF ? mr : 0.f;
+            float s_top = 0.f;
+#pragma unroll
+            for (int i = 0; i < NE; ++i) {
+                const bool top = f2i(qv[i]) >= 0;
+                v[i] = ex2((v[i] - (top ? m_top : m_rest)) * A.c2);
+                s_top += top ? v[i] : 0.f;
+                s_rest += top ? 0.f : v[i];
+            }
+            s_top = gsum<G>(s_top);
+            s_rest = gsum<G>(s_rest);
+            f_top = mt > ELG_NEG_INF ? ex2((m_top - m) * A.c2) : 0.f;
+            f_rest = mr > ELG_NEG_INF ? ex2((m_rest - m) * A.c2) : 0.f;
+            S = s_top * f_top + s_rest * f_rest;
+        } else {
+            m = v[0];
+#pragma unroll
+            for (int i = 1; i < NE; ++i) m = fmaxf(m, v[i]);
+            m = gmax<G>(m);
+            const float ref = m > ELG_NEG_INF ? m : 0.f;
+            S = 0.f;
+#pragma unroll
+            for (int i = 0; i < NE; ++i) {
+                v[i] = ex2((v[i] - ref) * A.c2);
+                S += v[i];
+            }
+            S = gsum<G>(S);
+        }
+        const bool live = on && !(S <= 0.f) && !(st <= 0.f);
+        const float inv_S = __builtin_amdgcn_rcpf(S);
+        // ---- loss
+        if (A.loss_rows || A.part) {
+            float L = 0.f;
+#pragma unroll
+            for (int e = 0; e < KE; ++e) L += q[e] > 0.f || q[e] != q[e] ? q[e] * ((et[e] - tm) - (zi[e] - m)) : 0.f;
+            L = gsum<G>(L) * inv_tau;
+            if (a < 1.f) L += (1.f - a) * ln(qscale * S);
+            if (TAIL && a > TINY_MASS) L += a * (ln(a * S * __builtin_amdgcn_rcpf(s_rest)) - (m_rest - m) * inv_tau);
+            L = live ? L * (A.tau * A.tau * w) : 0.f;
+            if (l == 0 && valid) {
+                if (A.loss_rows) A.loss_rows[r] = L * A.scale;
+                lacc += (double)L;
+            }
+        }
+        // ---- gradient
+        if (A.grad && valid) {
+            const float cot = A.cot ? A.cot[r * A.cot_stride] : 1.f;
+            const float Gr = live ? A.scale * cot * w * A.tau : 0.f, c_top = live ? Gr * f_top * inv_S : 0.f;
+            float c_rest = c_top;
+            if (TAIL) c_rest = live ? Gr * (f_rest * inv_S - (a > 0.f && s_rest > 0.f ? a * __builtin_amdgcn_rcpf(s_rest) : 0.f)) : 0.f;
+            elem_t<DT>* grow = reinterpret_cast<elem_t<DT>*>(A.grad + r * A.g_stride);
+#pragma unroll
+            for (int i = 0; i < NE; ++i) {
+                const float t = fmaf(live ? v[i] : 0.f, !TAIL || f2i(qv[i]) >= 0 ? c_top : c_rest, -Gr * qv[i]);
+                if (i * G + l < V) grow[i * G + l] = (elem_t<DT>)t;
+            }
+        }
+    }
+    if (A.part) {
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) lacc += __shfl_xor(lacc, d, 64);
+        if (lane == 0) dred[wave] = lacc;
+        __syncthreads();
+        if (threadIdx.x == 0) A.part[blockIdx.x] = (dred[0] + dred[1]) + (dred[2] + dred[3]);
+    }
+}
+
 // the workgroups' partial losses in workgroup order: the same bits in every run
 __global__ __launch_bounds__(256) void distill_total_kernel(const double* __restrict__ part, int n, float scale, float* __restrict__ total) {
     __shared__ double s[256];
@@ -224,6 +414,31 @@ __global__ __launch_bounds__(256) void distill_total_kernel(const double* __rest
 }
 
 constexpr int MAX_GRID = 2048;
+
+template <int DT, int G, int NE, int KE>
+void launch_small(const DistillArgs& A, int grid, hipStream_t s) {
+    if (A.tail) hipLaunchKernelGGL((distill_small_kernel<DT, G, NE, KE, true>), dim3((unsigned)grid), dim3(256), 0, s, A);
+    else hipLaunchKernelGGL((distill_small_kernel<DT, G, NE, KE, false>), dim3((unsigned)grid), dim3(256), 0, s, A);
+}
+
+// Rows of up to 256 logits take a quarter of a wave, up to 2048 a wave, longer ones a workgroup; the registers of a lane are sized by the
+// next power of two.
+template <int DT>
+int launch(const DistillArgs& A, hipStream_t s) {
+    const int V = A.V, k = A.k;
+    const long long rows_wg = V <= 256 ? 16 : V <= 2048 ? 4 : 1, want = (A.R + rows_wg - 1) / rows_wg;
+    const int grid = (int)(want < MAX_GRID ? want : MAX_GRID);
+    if (V <= 256) {
+        if (k > 48) V <= 128 ? launch_small<DT, 16, 8, 16>(A, grid, s) : launch_small<DT, 16, 16, 16>(A, grid, s);
+        else if (k > 16) V <= 64 ? launch_small<DT, 16, 4, 3>(A, grid, s) : V <= 128 ? launch_small<DT, 16, 8, 3>(A, grid, s) : launch_small<DT, 16, 16, 3>(A, grid, s);
+        else if (V <= 32) launch_small<DT, 16, 2, 1>(A, grid, s);
+        else V <= 64 ? launch_small<DT, 16, 4, 1>(A, grid, s) : V <= 128 ? launch_small<DT, 16, 8, 1>(A, grid, s) : launch_small<DT, 16, 16, 1>(A, grid, s);
+    } else if (V <= 2048) {
+        if (k <= 64) V <= 512 ? launch_small<DT, 64, 8, 1>(A, grid, s) : V <= 1024 ? launch_small<DT, 64, 16, 1>(A, grid, s) : launch_small<DT, 64, 32, 1>(A, grid, s);
+        else V <= 512 ? launch_small<DT, 64, 8, 4>(A, grid, s) : V <= 1024 ? launch_small<DT, 64, 16, 4>(A, grid, s) : launch_small<DT, 64, 32, 4>(A, grid, s);
+    } else hipLaunchKernelGGL((distill_row_kernel<DT, 256, 0>), dim3((unsigned)grid), dim3(256), 0, s, A);
+    return grid;
+}
 
 }  // namespace
 }  // namespace elg
@@ -260,12 +475,10 @@ extern "C" int elg_distill_loss_grad(const void* z, int64_t z_stride, int type, 
     A.loss_rows = loss_rows; A.part = loss_total ? (double*)ws : nullptr;
     A.grad = (char*)grad; A.g_stride = V * es;
     (void)hipGetLastError();
-    const int G = (int)(R < MAX_GRID ? R : MAX_GRID);
-    if (G > 0) {
-        const dim3 grid((unsigned)G);
-        if (type == ELG_F32) hipLaunchKernelGGL((distill_row_kernel<ELG_F32, 256, 0>), grid, dim3(256), 0, (hipStream_t)stream, A);
-        else if (type == ELG_BF16) hipLaunchKernelGGL((distill_row_kernel<ELG_BF16, 256, 0>), grid, dim3(256), 0, (hipStream_t)stream, A);
-        else hipLaunchKernelGGL((distill_row_kernel<ELG_F16, 256, 0>), grid, dim3(256), 0, (hipStream_t)stream, A);
+    int G = 0;
+    if (R > 0) {
+        hipStream_t st = (hipStream_t)stream;
+        G = type == ELG_F32 ? launch<ELG_F32>(A, st) : type == ELG_BF16 ? launch<ELG_BF16>(A, st) : launch<ELG_F16>(A, st);
     }
     if (loss_total) hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, (const double*)ws, G, scale, loss_total);
     return launch_status("distill");
