@@ -156,13 +156,10 @@ __device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x)
 // Order-preserving key of a float: larger value, larger key; -0 = +0; every NaN above +inf.
 constexpr unsigned KEY_NEG_INF = 0x007FFFFFu;
 __device__ __forceinline__ unsigned order_key(float f) {
-    const unsigned u = (unsigned)f2i(f);
-    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return 0xFFFFFFFFu;
-    if (u == 0x80000000u) return 0x80000000u;
-    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+    const int u = f2i(f + 0.0f);                                        // -0 + 0 = +0
+    return f != f ? 0xFFFFFFFFu : (unsigned)(u ^ ((u >> 31) | (int)0x80000000));
 }
-__device__ __forceinline__ float key_value(unsigned k) {
-    if (k == 0xFFFFFFFFu) return i2f(0x7FC00000);
-    return i2f((int)((k & 0x80000000u) ? k & 0x7FFFFFFFu : ~k));
+__device__ __forceinline__ float key_value(unsigned k) {               // (the NaN key gives back a NaN)
+    return i2f((int)k ^ ((~(int)k >> 31) | (int)0x80000000));
 }
 }  // namespace elg

@@ -23,6 +23,7 @@ struct TopArgs {
     char* values;
     int* idx;
     float* tail;
+    unsigned k_inv;                       // ceil(2^32 / k); 0 for k = 1
 };
 
 __device__ __forceinline__ unsigned long long composite(unsigned key, int n) {
@@ -205,6 +206,192 @@ __global__ __launch_bounds__(T) void top_row_kernel(const TopArgs A) {
     }
 }
 
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Short rows: a bitonic sort in registers, eight lanes to a row.  A lane holds NE positions of the order; merges across lanes go through
+// DPP alone (pairs, quads and mirrored halves of eight lanes are what it can reach in one step), merges inside a lane are plain registers.
+// The sort key is a whole composite in one comparable register: for 16-bit types a 32-bit integer (16 bits of value, 16 of index), for f32 a
+// double in [1, 2) whose 52 mantissa bits hold 32 of value and 20 of index -- v_max_f64 / v_min_f64 then order both at once, in two
+// instructions where a comparison with selects takes five.
+template <int DT>
+struct Key32 {
+    unsigned u;
+    static __device__ __forceinline__ Key32 make(float f, int n) {
+        const unsigned b = DT == ELG_BF16 ? (unsigned)f2i(f) >> 16 : (unsigned)__builtin_bit_cast(unsigned short, (_Float16)f);
+        unsigned key = (b & 0x8000u) ? ~b & 0xFFFFu : b | 0x8000u;
+        key = b == 0x8000u ? 0x8000u : key;                                   // -0 = +0
+        key = f != f ? 0xFFFFu : key;
+        return {key << 16 | (0xFFFFu - (unsigned)n)};
+    }
+    __device__ __forceinline__ float value() const {
+        const unsigned key = u >> 16, b = (key & 0x8000u) ? key & 0x7FFFu : ~key & 0xFFFFu;
+        return DT == ELG_BF16 ? i2f((int)(b << 16)) : (float)__builtin_bit_cast(_Float16, (unsigned short)b);
+    }
+    __device__ __forceinline__ int index() const { return (int)(0xFFFFu - (u & 0xFFFFu)); }
+    static __device__ __forceinline__ Key32 hi(Key32 a, Key32 b) { return {max(a.u, b.u)}; }
+    static __device__ __forceinline__ Key32 lo(Key32 a, Key32 b) { return {min(a.u, b.u)}; }
+    template <int CTRL> __device__ __forceinline__ Key32 moved() const { return {(unsigned)__builtin_amdgcn_mov_dpp((int)u, CTRL, 0xF, 0xF, true)}; }
+    __device__ __forceinline__ void raise(Key32 o) { asm("v_max_u32 %0, %0, %1" : "+v"(u) : "v"(o.u)); }
+    __device__ __forceinline__ void lower(Key32 o) { asm("v_min_u32 %0, %0, %1" : "+v"(u) : "v"(o.u)); }
+};
+struct Key64 {
+    double d;
+    static __device__ __forceinline__ Key64 of(unsigned long long mantissa) { return {__builtin_bit_cast(double, 0x3FF0000000000000ull | mantissa)}; }
+    static __device__ __forceinline__ Key64 make(float f, int n) { return of(((unsigned long long)order_key(f) << 20) | (0xFFFFFu - (unsigned)n)); }
+    __device__ __forceinline__ float value() const { return key_value((unsigned)(__builtin_bit_cast(unsigned long long, d) >> 20)); }
+    __device__ __forceinline__ int index() const { return (int)(0xFFFFFu - ((unsigned)__builtin_bit_cast(unsigned long long, d) & 0xFFFFFu)); }
+    // (asm: the library maximum first quiets operands that come out of integer registers -- these are never NaN)
+    static __device__ __forceinline__ Key64 hi(Key64 a, Key64 b) { Key64 r; asm("v_max_f64 %0, %1, %2" : "=v"(r.d) : "v"(a.d), "v"(b.d)); return r; }
+    static __device__ __forceinline__ Key64 lo(Key64 a, Key64 b) { Key64 r; asm("v_min_f64 %0, %1, %2" : "=v"(r.d) : "v"(a.d), "v"(b.d)); return r; }
+    template <int CTRL> __device__ __forceinline__ Key64 moved() const {
+        const unsigned long long u = __builtin_bit_cast(unsigned long long, d);
+        const unsigned l = (unsigned)__builtin_amdgcn_mov_dpp((int)(unsigned)u, CTRL, 0xF, 0xF, true);
+        const unsigned h = (unsigned)__builtin_amdgcn_mov_dpp((int)(unsigned)(u >> 32), CTRL, 0xF, 0xF, true);
+        return {__builtin_bit_cast(double, (unsigned long long)h << 32 | l)};
+    }
+    __device__ __forceinline__ void raise(Key64 o) { asm("v_max_f64 %0, %0, %1" : "+v"(d) : "v"(o.d)); }
+    __device__ __forceinline__ void lower(Key64 o) { asm("v_min_f64 %0, %0, %1" : "+v"(d) : "v"(o.d)); }
+};
+template <int DT> struct KeyOf { using K = Key32<DT>; };
+template <> struct KeyOf<ELG_F32> { using K = Key64; };
+
+// an odd-even merge sort's compare-exchanges
+template <int N> struct Network {
+    int a[N * 8] = {}, b[N * 8] = {}, n = 0;
+    constexpr Network() {
+        for (int p = 1; p < N; p *= 2)
+            for (int q = p; q >= 1; q /= 2)
+                for (int j = q % p; j + q < N; j += 2 * q)
+                    for (int i = 0; i < q && i + j + q < N; ++i)
+                        if ((i + j) / (2 * p) == (i + j + q) / (2 * p)) { a[n] = i + j; b[n] = i + j + q; ++n; }
+    }
+};
+
+template <class K, int NE>
+__device__ __forceinline__ void exchange(K (&x)[NE], int i, int j) {
+    const K a = x[i], b = x[j];
+    x[i] = K::hi(a, b);
+    x[j] = K::lo(a, b);
+}
+template <class K, int NE>
+__device__ __forceinline__ void merge_lane(K (&x)[NE]) {
+#pragma unroll
+    for (int d = NE / 2; d >= 1; d /= 2)
+#pragma unroll
+        for (int s = 0; s < NE; ++s)
+            if (!(s & d)) exchange(x, s, s + d);
+}
+// the lanes that keep the larger of their pairs, then the others: two moves and two ordered operations a value
+template <class K, int NE>
+__device__ __forceinline__ void keep(K (&x)[NE], const K (&y)[NE], bool up) {
+    if (up) {
+#pragma unroll
+        for (int s = 0; s < NE; ++s) x[s].raise(y[s]);
+    } else {
+#pragma unroll
+        for (int s = 0; s < NE; ++s) x[s].lower(y[s]);
+    }
+}
+template <int CTRL, class K, int NE>
+__device__ __forceinline__ void across_mirror(K (&x)[NE], bool up) {
+    K y[NE];
+#pragma unroll
+    for (int s = 0; s < NE; ++s) y[s] = x[NE - 1 - s].template moved<CTRL>();
+    keep(x, y, up);
+}
+template <int CTRL, class K, int NE>
+__device__ __forceinline__ void across(K (&x)[NE], bool up) {
+    K y[NE];
+#pragma unroll
+    for (int s = 0; s < NE; ++s) y[s] = x[s].template moved<CTRL>();
+    keep(x, y, up);
+}
+
+constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_MIRROR4 = 0x1B, DPP_MIRROR8 = 0x141;
+
+// 8 rows to a wave, 4 waves to a workgroup (2 where 4 would need over 64 KB of LDS); waves never wait for each other.  LDS turns the lanes' runs of the order into the rows' packed output.
+template <int DT, int NE>
+__global__ __launch_bounds__(256, NE == 32 ? 3 : 4) void top_sort_kernel(const TopArgs A) {
+    using K = typename KeyOf<DT>::K;
+    extern __shared__ __attribute__((aligned(16))) unsigned char top_lds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, g = lane >> 3, l = lane & 7, V = A.V, k = A.k;
+    const int lanes_out = (k + NE - 1) / NE;               // lanes of a row that hold winners; a lane's run is padded by one against bank conflicts
+    K* out = reinterpret_cast<K*>(top_lds) + wave * 8 * lanes_out * (NE + 1);
+    constexpr Network<NE> net{};
+    for (long long r0 = ((long long)blockIdx.x * waves + wave) * 8; r0 < A.R; r0 += (long long)gridDim.x * waves * 8) {
+        const long long r = r0 + g;
+        const bool valid = r < A.R;
+        const elem_t<DT>* row = reinterpret_cast<const elem_t<DT>*>(A.z + (valid ? r : r0) * A.stride_bytes) + l;
+        int n0 = l;
+        asm volatile("" : "+v"(n0));      // the slots' node numbers are formed here, not kept in registers across the rows
+        K x[NE];
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+            float f = ELG_NEG_INF;                            // behind every node of the row: a closed one of a higher index
+            if (i * 8 + 8 <= V) f = (float)row[i * 8];
+            else if (i * 8 < V && i * 8 + n0 < V) f = (float)row[i * 8];
+            x[i] = K::make(f, i * 8 + n0);
+        }
+#pragma unroll
+        for (int c = 0; c < net.n; ++c) exchange(x, net.a[c], net.b[c]);
+        across_mirror<DPP_XOR1>(x, !(l & 1));
+        merge_lane(x);
+        across_mirror<DPP_MIRROR4>(x, !(l & 2));
+        across<DPP_XOR1>(x, !(l & 1));
+        merge_lane(x);
+        across_mirror<DPP_MIRROR8>(x, !(l & 4));
+        across<DPP_XOR2>(x, !(l & 2));
+        across<DPP_XOR1>(x, !(l & 1));
+        merge_lane(x);
+        // position l NE + s of the order is slot s of lane l
+        if (A.tail) {
+            const float m = __shfl(x[0].value(), lane & 56, 64);
+            float top = 0.f, rest = 0.f;
+            const int k_here = k - n0 * NE;          // of this lane's positions, how many are among the k
+#pragma unroll
+            for (int s = 0; s < NE; ++s) {
+                const float e = ex2((x[s].value() - m) * A.c2);
+                top += s < k_here ? e : 0.f;
+                rest += s < k_here ? 0.f : e;
+            }
+            top = oct_sum(top);
+            rest = oct_sum(rest);
+            // a row without an open node gives (-inf) - (-inf) = NaN here
+            if (l == 0 && valid) A.tail[r] = m > ELG_NEG_INF || m != m ? rest * __builtin_amdgcn_rcpf(top + rest) : 0.f;
+        }
+        wave_lds_fence();
+        if (n0 * NE < k) {
+#pragma unroll
+            for (int s = 0; s < NE; ++s) out[(g * lanes_out + n0) * (NE + 1) + s] = x[s];
+        }
+        wave_lds_fence();
+        const int n_out = (int)(A.R - r0 < 8 ? A.R - r0 : 8) * k;
+        for (int f = lane; f < n_out; f += 64) {
+            const int og = k > 1 ? (int)__umulhi((unsigned)f, A.k_inv) : f, pos = f - og * k;            // f / k: exact for f < 2^11
+            const K w = out[(og * lanes_out + pos / NE) * (NE + 1) + pos % NE];
+            reinterpret_cast<elem_t<DT>*>(A.values)[r0 * k + f] = (elem_t<DT>)w.value();
+            A.idx[r0 * k + f] = w.index();
+        }
+        wave_lds_fence();
+    }
+}
+
+template <int DT, int NE>
+void launch_sort(const TopArgs& A, hipStream_t s) {
+    const size_t per_wave = (size_t)8 * ((A.k + NE - 1) / NE) * (NE + 1) * sizeof(typename KeyOf<DT>::K);
+    const int waves = 4 * per_wave > 65536 ? 2 : 4;
+    const long long want = (A.R + waves * 8 - 1) / (waves * 8);
+    hipLaunchKernelGGL((top_sort_kernel<DT, NE>), dim3((unsigned)(want < 4096 ? want : 4096)), dim3(64 * waves), waves * per_wave, s, A);
+}
+
+template <int DT>
+void launch_top(const TopArgs& A, hipStream_t s) {
+    if (A.V <= 32) launch_sort<DT, 4>(A, s);
+    else if (A.V <= 64) launch_sort<DT, 8>(A, s);
+    else if (A.V <= 128) launch_sort<DT, 16>(A, s);
+    else if (A.V <= 256) launch_sort<DT, 32>(A, s);
+    else hipLaunchKernelGGL((top_row_kernel<DT, 256>), dim3((unsigned)(A.R < 16384 ? A.R : 16384)), dim3(256), 0, s, A);
+}
+
 }  // namespace
 }  // namespace elg
 
@@ -225,11 +412,10 @@ extern "C" int elg_top_logits(const void* z, int64_t z_stride, int type, int64_t
     A.stride_bytes = z_stride * es;
     A.R = R; A.V = (int)V; A.k = k;
     A.c2 = LOG2E / temperature;
+    A.k_inv = k > 1 ? (unsigned)((0x100000000ull + k - 1) / k) : 0u;
     A.values = (char*)values; A.idx = idx; A.tail = tail;
     (void)hipGetLastError();
-    const dim3 grid((unsigned)(R < 16384 ? R : 16384));
-    if (type == ELG_F32) hipLaunchKernelGGL((top_row_kernel<ELG_F32, 256>), grid, dim3(256), 0, (hipStream_t)stream, A);
-    else if (type == ELG_BF16) hipLaunchKernelGGL((top_row_kernel<ELG_BF16, 256>), grid, dim3(256), 0, (hipStream_t)stream, A);
-    else hipLaunchKernelGGL((top_row_kernel<ELG_F16, 256>), grid, dim3(256), 0, (hipStream_t)stream, A);
+    hipStream_t st = (hipStream_t)stream;
+    type == ELG_F32 ? launch_top<ELG_F32>(A, st) : type == ELG_BF16 ? launch_top<ELG_BF16>(A, st) : launch_top<ELG_F16>(A, st);
     return launch_status("top_logits");
 }
