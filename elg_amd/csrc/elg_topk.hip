@@ -8,6 +8,7 @@
 // gathered into LDS (any order) and ranked by counting: rank = number of larger composites.  Rows that defeat the bound (thousands of equal
 // values) fall back to a bisection over the keys of all elements, with equal values taken in index order.
 #include "elg_logits.h"
+#include <type_traits>
 
 namespace elg {
 namespace {
@@ -70,8 +71,8 @@ struct Count {                            // block-wide counts; one barrier each
     }
 };
 
-// One workgroup per row; the row is read again (from L2) by every pass.
-template <int DT, int T>
+// One workgroup per row.  C > 0: the row stays in registers, C chunks a thread; C = 0: every pass reads it again.
+template <int DT, int T, int C>
 __global__ __launch_bounds__(T) void top_row_kernel(const TopArgs A) {
     __shared__ unsigned long long cand[TOP_CAP];
     __shared__ unsigned long long win[ELG_TOP_MAX_K];
@@ -84,14 +85,33 @@ __global__ __launch_bounds__(T) void top_row_kernel(const TopArgs A) {
     for (long long r = blockIdx.x; r < A.R; r += gridDim.x) {
         const char* row = A.z + r * A.stride_bytes;
         const int shift = shift_of<DT>(row), nch = (shift + V + VEC<DT> - 1) / VEC<DT>;
-        auto each = [&](auto&& f) {       // f(key, index) for every element of this thread, closed nodes included
-            for (int c = tid; c < nch; c += T) {
-                float v[VEC<DT>];
-                unpack<DT>(load_chunk<DT>(row, shift, V, c, 0u), v);
+        u32x4 zr[C ? C : 1];
+        if (C) {
 #pragma unroll
-                for (int e = 0; e < VEC<DT>; ++e) {
-                    const int n = c * VEC<DT> + e - shift;
-                    if (n >= 0 && n < V) f(order_key(v[e]), n);
+            for (int c = 0; c < C; ++c) {
+                constexpr unsigned pad = PAD_NEG_INF<DT>;
+                zr[c] = tid + c * T < nch ? load_chunk<DT>(row, shift, V, tid + c * T, pad) : u32x4{pad, pad, pad, pad};
+            }
+        }
+        // f(key, index) for every element of this thread; positions outside the row come as closed nodes
+        auto each = [&](auto&& f) {
+            if (C) {
+                int n0 = tid * VEC<DT> - shift;
+                asm volatile("" : "+v"(n0));          // node numbers are formed where they are used, not kept in registers for the next pass
+#pragma unroll
+                for (int c = 0; c < C; ++c) {
+                    float v[VEC<DT>];
+                    asm volatile("" : "+v"(zr[c]));   // and so are the keys
+                    unpack<DT>(zr[c], v);
+#pragma unroll
+                    for (int e = 0; e < VEC<DT>; ++e) f(order_key(v[e]), n0 + c * T * VEC<DT> + e);
+                }
+            } else {
+                for (int c = tid; c < nch; c += T) {
+                    float v[VEC<DT>];
+                    unpack<DT>(load_chunk<DT>(row, shift, V, c, PAD_NEG_INF<DT>), v);
+#pragma unroll
+                    for (int e = 0; e < VEC<DT>; ++e) f(order_key(v[e]), c * VEC<DT> + e - shift);
                 }
             }
         };
@@ -248,6 +268,7 @@ struct Key64 {
         const unsigned h = (unsigned)__builtin_amdgcn_mov_dpp((int)(unsigned)(u >> 32), CTRL, 0xF, 0xF, true);
         return {__builtin_bit_cast(double, (unsigned long long)h << 32 | l)};
     }
+    static __device__ __forceinline__ Key64 pick(bool up, Key64 a, Key64 b) { return (a.d > b.d) == up ? a : b; }
     __device__ __forceinline__ void raise(Key64 o) { asm("v_max_f64 %0, %0, %1" : "+v"(d) : "v"(o.d)); }
     __device__ __forceinline__ void lower(Key64 o) { asm("v_min_f64 %0, %0, %1" : "+v"(d) : "v"(o.d)); }
 };
@@ -383,13 +404,257 @@ void launch_sort(const TopArgs& A, hipStream_t s) {
     hipLaunchKernelGGL((top_sort_kernel<DT, NE>), dim3((unsigned)(want < 4096 ? want : 4096)), dim3(64 * waves), waves * per_wave, s, A);
 }
 
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Rows of 257 to 2048 logits: a wave to a row, lane l holding the nodes i 64 + l.  The same selection as a workgroup's below, with counts by
+// ballot: a bound from the maxima of groups of NE / 4 nodes, the few candidates above it compacted through LDS, then sorted with one, two or
+// four to a lane.
+template <int NE>
+struct WaveRow {
+    unsigned key[NE];
+    // number of the row's keys >= t, the same in every lane
+    __device__ __forceinline__ int count(unsigned t) const {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < NE; ++i) c += __popcll(__ballot(key[i] >= t));
+        return c;
+    }
+};
+
+// lane i <- lane i ^ D, D = 4 and 8 by two mirrors, 16 and 32 by the lane swaps
+template <int D>
+__device__ __forceinline__ Key64 lane_xor(const Key64 k) {
+    if constexpr (D == 1) return k.moved<DPP_XOR1>();
+    else if constexpr (D == 2) return k.moved<DPP_XOR2>();
+    else if constexpr (D == 4) return k.moved<DPP_MIRROR8>().template moved<DPP_MIRROR4>();
+    else if constexpr (D == 8) return k.moved<0x128>();                      // row_ror:8
+    else {
+        const unsigned long long u = __builtin_bit_cast(unsigned long long, k.d);
+        const unsigned lo = (unsigned)u, hi = (unsigned)(u >> 32);
+        if constexpr (D == 16) {
+            const u32x2_t a = __builtin_amdgcn_permlane16_swap(lo, lo, false, false), b = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+            const bool odd = threadIdx.x & 16;
+            const unsigned l2 = odd ? a[0] : a[1], h2 = odd ? b[0] : b[1];
+            return {__builtin_bit_cast(double, (unsigned long long)h2 << 32 | l2)};
+        } else {
+            const u32x2_t a = __builtin_amdgcn_permlane32_swap(lo, lo, false, false), b = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+            const bool odd = threadIdx.x & 32;
+            const unsigned l2 = odd ? a[0] : a[1], h2 = odd ? b[0] : b[1];
+            return {__builtin_bit_cast(double, (unsigned long long)h2 << 32 | l2)};
+        }
+    }
+}
+// position lane * E + s of the descending order, E elements to a lane; bitonic, every merge in one direction per block of lanes
+template <int E, int D>
+__device__ __forceinline__ void merge_lanes(Key64 (&x)[E], int lane, bool down) {
+#pragma unroll
+    for (int s = 0; s < E; ++s) {
+        const Key64 o = lane_xor<D>(x[s]);
+        x[s] = Key64::pick(!(lane & D) != down, x[s], o);
+    }
+    if constexpr (D > 1) merge_lanes<E, D / 2>(x, lane, down);
+}
+template <int E>
+__device__ __forceinline__ void merge_slots(Key64 (&x)[E], bool down) {
+#pragma unroll
+    for (int d = E / 2; d >= 1; d /= 2)
+#pragma unroll
+        for (int s = 0; s < E; ++s)
+            if (!(s & d)) {
+                const Key64 a = x[s], b = x[s + d], h = Key64::hi(a, b), l = Key64::lo(a, b);
+                x[s] = down ? l : h;
+                x[s + d] = down ? h : l;
+            }
+}
+template <int E, int D>
+__device__ __forceinline__ void sort_lanes(Key64 (&x)[E], int lane) {
+    if constexpr (D > 1) sort_lanes<E, D / 2>(x, lane);
+    // blocks of 2 D lanes alternate in direction (the last block is the whole wave: descending)
+    const bool down = D < 32 && (lane & (2 * D));
+    merge_lanes<E, D>(x, lane, down);
+    merge_slots<E>(x, down);
+}
+template <int E>
+__device__ __forceinline__ void sort_wave(Key64 (&x)[E], int lane) {
+    if constexpr (E > 1) {
+#pragma unroll
+        for (int p = 2; p <= E; p *= 2)
+#pragma unroll
+            for (int d = p / 2; d >= 1; d /= 2)
+#pragma unroll
+                for (int s = 0; s < E; ++s)
+                    if (!(s & d)) {
+                        const Key64 a = x[s], b = x[s + d], h = Key64::hi(a, b), l = Key64::lo(a, b);
+                        const bool rev = p < E ? (s & p) != 0 : (lane & 1);
+                        x[s] = rev ? l : h;
+                        x[s + d] = rev ? h : l;
+                    }
+    }
+    sort_lanes<E, 32>(x, lane);
+}
+
+template <int DT, int NE>
+__global__ __launch_bounds__(256) void top_wave_kernel(const TopArgs A) {
+    constexpr int CAP = 256, GR = 4;                       // candidates a wave can sort; groups of nodes a lane keeps maxima of
+    __shared__ double cand_all[4 * CAP];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, V = A.V, k = A.k;
+    Key64* cand = reinterpret_cast<Key64*>(cand_all) + wave * CAP;
+    for (long long r = (long long)blockIdx.x * 4 + wave; r < A.R; r += (long long)gridDim.x * 4) {
+        const elem_t<DT>* row = reinterpret_cast<const elem_t<DT>*>(A.z + r * A.stride_bytes) + lane;
+        int n0 = lane;
+        asm volatile("" : "+v"(n0));              // node numbers and their comparisons are formed where they are used, not kept across the rows
+        WaveRow<NE> z;
+#pragma unroll
+        for (int i = 0; i < NE; ++i) {
+            float f = ELG_NEG_INF;
+            if (n0 < V - i * 64) f = (float)row[i * 64];
+            z.key[i] = order_key(f);
+        }
+        unsigned gm[GR], best = 0;
+#pragma unroll
+        for (int g = 0; g < GR; ++g) {
+            gm[g] = z.key[g * (NE / GR)];
+#pragma unroll
+            for (int i = 1; i < NE / GR; ++i) gm[g] = max(gm[g], z.key[g * (NE / GR) + i]);
+            best = max(best, gm[g]);
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) best = max(best, (unsigned)__shfl_xor((int)best, d, 64));
+        auto groups = [&](unsigned t) {
+            int c = 0;
+#pragma unroll
+            for (int g = 0; g < GR; ++g) c += __popcll(__ballot(gm[g] >= t));
+            return c;
+        };
+        // ---- a lower bound of the k-th best: the k-th best group maximum (open nodes only)
+        unsigned lo = KEY_NEG_INF + 1, hi = best;
+        if (groups(lo) >= k)
+            while (lo < hi) {
+                const unsigned mid = lo + (hi - lo) / 2 + 1;
+                const int c = groups(mid);
+                if (c >= k) {
+                    lo = mid;
+                    if (c == k) break;
+                } else hi = mid - 1;
+            }
+        int found = z.count(lo), ties = 0;
+        unsigned tie_key = 0;
+        if (found > CAP) {                                 // too many: the k-th best key itself, then equal ones by index
+            hi = best;
+            while (lo < hi) {
+                const unsigned mid = lo + (hi - lo) / 2 + 1;
+                const int c = z.count(mid);
+                if (c >= k) {
+                    lo = mid;
+                    if (c == k) break;
+                } else hi = mid - 1;
+            }
+            tie_key = lo;
+            found = lo < 0xFFFFFFFFu ? z.count(lo + 1) : 0;
+            ties = k - found;
+            ++lo;                                          // (NaN as the tie: lo wraps to 0, and nothing is above it)
+            if (tie_key == 0xFFFFFFFFu) lo = 0xFFFFFFFFu;
+        } else if (found < k) {                            // closed nodes fill the rest, by index
+            tie_key = KEY_NEG_INF;
+            ties = k - found;
+        }
+        // ---- compaction: nodes above the bound in any order, then the ties in index order
+        wave_lds_fence();
+        int at = 0;
+        if (found > 0)
+#pragma unroll
+            for (int i = 0; i < NE; ++i) {
+                const bool hit = z.key[i] >= lo && !(ties > 0 && z.key[i] == tie_key);
+                const unsigned long long m = __ballot(hit);
+                if (hit) cand[at + lanes_below(m)] = Key64::of(((unsigned long long)z.key[i] << 20) | (0xFFFFFu - (unsigned)(i * 64 + n0)));
+                at += __popcll(m);
+            }
+        int need = ties;
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+            if (need > 0) {
+                const bool hit = z.key[i] == tie_key && n0 < V - i * 64;
+                const unsigned long long m = __ballot(hit);
+                const int b = lanes_below(m);
+                if (hit && b < need) cand[at + b] = Key64::of(((unsigned long long)z.key[i] << 20) | (0xFFFFFu - (unsigned)(i * 64 + n0)));
+                const int n = min(need, (int)__popcll(m));
+                at += n;
+                need -= n;
+            }
+        wave_lds_fence();
+        // ---- order
+        Key64 last;                                        // the k-th best
+        auto finish = [&](auto tag) {
+            constexpr int E = decltype(tag)::value;
+            Key64 x[E];
+#pragma unroll
+            for (int s = 0; s < E; ++s) x[s] = s * 64 + lane < at ? cand[s * 64 + lane] : Key64::of(0);
+            sort_wave<E>(x, lane);
+            wave_lds_fence();
+#pragma unroll
+            for (int s = 0; s < E; ++s)
+                if (lane * E + s < k) cand[lane * E + s] = x[s];
+            wave_lds_fence();
+        };
+        if (at <= 64) finish(std::integral_constant<int, 1>{});
+        else if (at <= 128) finish(std::integral_constant<int, 2>{});
+        else finish(std::integral_constant<int, 4>{});
+        for (int i = lane; i < k; i += 64) {
+            const Key64 w = cand[i];
+            reinterpret_cast<elem_t<DT>*>(A.values)[r * k + i] = (elem_t<DT>)w.value();
+            A.idx[r * k + i] = w.index();
+        }
+        last = cand[k - 1];
+        if (A.tail) {
+            const float m = key_value(best);
+            const unsigned long long lu = __builtin_bit_cast(unsigned long long, last.d) & 0xFFFFFFFFFFFFFull;
+            const unsigned lkey = (unsigned)(lu >> 20);
+            const int lidx = last.index();
+            float top = 0.f, rest = 0.f;
+#pragma unroll
+            for (int i = 0; i < NE; ++i) {
+                const float e = ex2((key_value(z.key[i]) - m) * A.c2);
+                const bool in = z.key[i] > lkey || (z.key[i] == lkey && n0 <= lidx - i * 64);
+                top += in ? e : 0.f;
+                rest += in ? 0.f : e;
+            }
+            top = wave_sum(top);
+            rest = wave_sum(rest);
+            if (lane == 0) A.tail[r] = m > ELG_NEG_INF || m != m ? rest * __builtin_amdgcn_rcpf(top + rest) : 0.f;
+        }
+        wave_lds_fence();
+    }
+}
+
+template <int DT, int T, int C>
+void launch_row(const TopArgs& A, hipStream_t s) {
+    const long long cap = 2048 * 256 / T;                  // workgroups: what the chip holds at once
+    hipLaunchKernelGGL((top_row_kernel<DT, T, C>), dim3((unsigned)(A.R < cap ? A.R : cap)), dim3(T), 0, s, A);
+}
+template <int DT, int NE>
+void launch_wave(const TopArgs& A, hipStream_t s) {
+    const long long want = (A.R + 3) / 4;
+    hipLaunchKernelGGL((top_wave_kernel<DT, NE>), dim3((unsigned)(want < 2048 ? want : 2048)), dim3(256), 0, s, A);
+}
+
+// Up to 256 logits: sorted, eight lanes a row.  Up to 2048: selected, a wave a row.  Longer: a workgroup a row, its size and the chunks a
+// thread holds by what keeps the row in registers (up to 256 KB of them); beyond that the row is read by every pass.
 template <int DT>
 void launch_top(const TopArgs& A, hipStream_t s) {
+    const bool aligned = !((uintptr_t)A.z & 15) && !(A.stride_bytes & 15);
+    const int nch = (A.V + (aligned ? 0 : VEC<DT> - 1) + VEC<DT> - 1) / VEC<DT>;
     if (A.V <= 32) launch_sort<DT, 4>(A, s);
     else if (A.V <= 64) launch_sort<DT, 8>(A, s);
     else if (A.V <= 128) launch_sort<DT, 16>(A, s);
     else if (A.V <= 256) launch_sort<DT, 32>(A, s);
-    else hipLaunchKernelGGL((top_row_kernel<DT, 256>), dim3((unsigned)(A.R < 16384 ? A.R : 16384)), dim3(256), 0, s, A);
+    else if (A.V <= 512) launch_wave<DT, 8>(A, s);
+    else if (A.V <= 1024) launch_wave<DT, 16>(A, s);
+    else if (A.V <= 2048) launch_wave<DT, 32>(A, s);
+    else if (nch <= 256 * 4) launch_row<DT, 256, 4>(A, s);
+    else if (nch <= 256 * 8) launch_row<DT, 256, 8>(A, s);
+    else if (nch <= 512 * 8) launch_row<DT, 512, 8>(A, s);
+    else if (nch <= 1024 * 8) launch_row<DT, 1024, 8>(A, s);
+    else if (nch <= 1024 * 16) launch_row<DT, 1024, 16>(A, s);
+    else launch_row<DT, 1024, 0>(A, s);
 }
 
 }  // namespace
