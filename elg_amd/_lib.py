@@ -108,7 +108,7 @@ EXPORTS = ["elg_version", "elg_last_error", "elg_aug8", "elg_dist_matrix", "elg_
            "elg_local_fold_fwd", "elg_local_fold_bwd", "elg_check_feasible", "elg_rollout_stats", "elg_decoder_bwd",
            "elg_decoder_bwd_ws_floats",
            "elg_rollout_scratch_floats", "elg_rollout_last_kernel",
-           "elg_top_logits", "elg_distill_ws_bytes", "elg_distill_loss_grad", "elg_verify_draft"]
+           "elg_top_logits", "elg_distill_ws_bytes", "elg_distill_loss_grad", "elg_verify_ws_bytes", "elg_verify_draft"]
 
 _lib = None
 
@@ -170,7 +170,9 @@ def lib() -> C.CDLL:
         L.elg_distill_ws_bytes.argtypes = [i64, i64, i]
         L.elg_distill_ws_bytes.restype = i64
         L.elg_distill_loss_grad.argtypes = [f, i64, i, i64, i64, f, i, f, i, i, f, fl, f, f, i, fl, f, f, f, f, i64, f]
-        L.elg_verify_draft.argtypes = [f, i64, i64, f, i64, i64, i, f, i, i64, f, i64, f, i64, i, i64, f, f, f]
+        L.elg_verify_ws_bytes.argtypes = [i64, i64, i]
+        L.elg_verify_ws_bytes.restype = i64
+        L.elg_verify_draft.argtypes = [f, i64, i64, f, i64, i64, i, f, i, i64, f, i64, f, i64, i, i64, f, f, f, i64, f]
         L.elg_check_feasible.restype = C.c_int
         L.elg_rollout_stats.restype = C.c_int
         L.elg_local_fold_fwd.restype = C.c_int

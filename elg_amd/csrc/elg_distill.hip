@@ -38,178 +38,382 @@ struct DistillArgs {
 constexpr float TINY_MASS = 1e-36f;       // a (log a - log p_rest) below this is nothing in f32
 __device__ __forceinline__ float ln(float x) { return __builtin_amdgcn_logf(x) * 0.6931471805599453f; }
 
-constexpr int SEG = 65536;                // window positions whose membership bits are held at a time
+// ---------------------------------------------------------------------------------------------------------------------------------
+// Long rows: T >= ELG_TOP_MAX_K threads, thread j < k holding entry j, the row in 16-byte chunks.  A bitmap in LDS tells a chunk which of its
+// nodes are entries': they stay out of the rest's sum, are written like the others and then written over.
 
-// One workgroup per row, T >= ELG_TOP_MAX_K threads: thread j < k holds entry j.  C > 0: the row stays in registers, C chunks a thread;
-// C = 0: it is read once for the sums and once for the gradient.
+// entry j = threadIdx.x of row r
+struct Entry {
+    int i = -1;                           // its node
+    float t = ELG_NEG_INF, z = ELG_NEG_INF;
+    __device__ __forceinline__ void load(const DistillArgs& A, long long r) {
+        if ((int)threadIdx.x >= A.k) return;
+        const long long at = r * A.k + threadIdx.x, n = index_any(A.ti, at, A.ti_wide);
+        if (n >= 0 && n < A.V) {
+            i = (int)n;
+            t = elem_any(A.tv, at, A.tv_type);
+        }
+    }
+    template <int DT> __device__ __forceinline__ void gather(const void* row) { if (i >= 0) z = elem<DT>(row, i); }
+    // is this the first entry of its node (first), and is it the only one?  idx: the row's nodes in LDS, padded to fours with -2
+    __device__ __forceinline__ void twins(const int* idx, int k, bool& first, bool& only) const {
+        first = only = i >= 0;
+        if (i < 0) return;
+        const int me = threadIdx.x;
+        for (int j = 0; j < k; j += 4) {
+            const int4 o = *reinterpret_cast<const int4*>(idx + j);
+            const unsigned m = (o.x == i) | (o.y == i) << 1 | (o.z == i) << 2 | (o.w == i) << 3;
+            const unsigned own = (me >> 2) == (j >> 2) ? 1u << (me & 3) : 0u;
+            only = only && (m & ~own) == 0u;
+            first = first && (j > me || (m & (own ? own - 1u : 15u)) == 0u);
+        }
+    }
+};
+
+// What a row comes down to, given its maxima and sums; the same in every thread.
+struct RowScalars {
+    bool live;
+    float loss, q_scale, m, inv_S, c_rest, m_rest, G;
+    // mt, mz, mr: largest teacher logit, entry's logit, other logit (-inf: none); st, sz, sr: sums of exponentials relative to each;
+    // sd: sum over entries of e^((t - mt) / tau) ((t - mt) - (z - m))
+    __device__ __forceinline__ RowScalars(const DistillArgs& A, long long r, float w, float mt, float mz, float mr, float st, float sz, float sr, float sd) {
+        float a = A.tail ? A.tail[r] : 0.f;
+        a = a > 1.f ? 1.f : a < 0.f ? 0.f : a;
+        m = fmaxf(mz, mr);
+        m_rest = mr > ELG_NEG_INF ? mr : 0.f;
+        const float f_top = mz > ELG_NEG_INF ? ex2((mz - m) * A.c2) : 0.f, f_rest = mr > ELG_NEG_INF ? ex2((mr - m) * A.c2) : 0.f;
+        const float S = sz * f_top + sr * f_rest;
+        live = !(S <= 0.f) && !(st <= 0.f);
+        inv_S = __builtin_amdgcn_rcpf(S);
+        q_scale = st <= 0.f ? 0.f : (1.f - a) * __builtin_amdgcn_rcpf(st);
+        const float inv_tau = 1.f / A.tau;
+        float L = sd * q_scale * inv_tau;
+        if (a < 1.f) L += (1.f - a) * ln(q_scale * S);
+        if (a > TINY_MASS) L += a * (ln(a * S * __builtin_amdgcn_rcpf(sr)) - (m_rest - m) * inv_tau);
+        loss = live ? L * (A.tau * A.tau * w) : 0.f;
+        const float cot = A.cot ? A.cot[r * A.cot_stride] : 1.f;
+        G = live ? A.scale * cot * w * A.tau : 0.f;
+        c_rest = live ? G * (f_rest * inv_S - (a > 0.f && sr > 0.f ? a * __builtin_amdgcn_rcpf(sr) : 0.f)) : 0.f;
+    }
+};
+
+// N sums or maxima over the workgroup: one LDS exchange, one barrier; buffers alternate
+template <int W, int N>
+struct BlockN {
+    float* buf;                           // 2 * W * N floats
+    int flip = 0;
+    __device__ explicit BlockN(float* b) : buf(b) {}
+    template <bool MAX> __device__ __forceinline__ void run(float (&v)[N]) {
+        float* s = buf + flip * W * N;
+        flip ^= 1;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            v[i] = MAX ? wave_max(v[i]) : wave_sum(v[i]);
+            if ((threadIdx.x & 63) == 0) s[(threadIdx.x >> 6) * N + i] = v[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = s[i];
+        for (int w = 1; w < W; ++w)
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = MAX ? fmaxf(v[i], s[w * N + i]) : v[i] + s[w * N + i];
+    }
+};
+
+// running maximum and sum of exponentials of the nodes that are no entry's, a few chunks at a time
+struct Rest {
+    float m = ELG_NEG_INF, s = 0.f;
+    template <int N> __device__ __forceinline__ void add(const float (&v)[N], float c2) {
+        float cm = v[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) cm = fmaxf(cm, v[i]);
+        if (cm > m) {
+            s = m > ELG_NEG_INF ? s * ex2((m - cm) * c2) : s;
+            m = cm;
+        }
+        const float ref = m > ELG_NEG_INF ? m : 0.f;
+        float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < N; ++i) t[i & 3] += ex2((v[i] - ref) * c2);
+        s += (t[0] + t[1]) + (t[2] + t[3]);
+        asm volatile("" : "+v"(s), "+v"(m));          // finished before the next values are unpacked
+    }
+    __device__ __forceinline__ float to(float all, float c2) const { return m > ELG_NEG_INF ? s * ex2((m - all) * c2) : s; }
+};
+
+template <int DT>
+__device__ __forceinline__ void hide_entries(float (&v)[VEC<DT>], unsigned b) {
+    if (__any(b & ((1u << VEC<DT>) - 1u)))            // most chunks hold none
+#pragma unroll
+        for (int e = 0; e < VEC<DT>; ++e) v[e] = (b >> e) & 1u ? ELG_NEG_INF : v[e];
+}
+// the gradient of a chunk, all its nodes taken as the rest's
+template <int DT>
+__device__ __forceinline__ void rest_grad(float (&v)[VEC<DT>], const RowScalars& s, float c2) {
+#pragma unroll
+    for (int e = 0; e < VEC<DT>; ++e) v[e] = s.live ? ex2((v[e] - s.m_rest) * c2) * s.c_rest : 0.f;
+}
+template <int DT>
+__device__ __forceinline__ void entry_grad(void* grow, const Entry& en, const int* idx, const float* ee, int k, bool only, const RowScalars& s, float c2, float mine) {
+    float q = mine;
+    if (!only) {                                      // the node's masses in entry order
+        q = 0.f;
+        for (int j = 0; j < k; ++j) q += idx[j] == en.i ? ee[j] : 0.f;
+    }
+    reinterpret_cast<elem_t<DT>*>(grow)[en.i] = (elem_t<DT>)(s.G * (ex2((en.z - s.m) * c2) * s.inv_S - q * s.q_scale));
+}
+
+// zero or the rest's gradient into the chunks [c_lo, c_hi) that thread t owns, t + i step, i < C, and its edge element
+template <int DT, int C>
+__device__ __forceinline__ void store_rest(char* grow, const Span<DT>& sp, int t, int step, int c_hi, u32x4 (&zr)[C], int edge, float ze, const RowScalars& s, float c2) {
+    const bool wide = shift_of<DT>(grow) == sp.shift;          // the gradient's rows lie like the logits': whole chunks
+    elem_t<DT>* g0 = reinterpret_cast<elem_t<DT>*>(grow);
+    char* gbase = grow - ((uintptr_t)grow & 15);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int at = t + c * step;
+        if (at >= c_hi) break;
+        float v[VEC<DT>];
+        asm volatile("" : "+v"(zr[c]));       // unpacked again, not kept unpacked
+        unpack<DT>(zr[c], v);
+        rest_grad<DT>(v, s, c2);
+        if (at >= sp.c_lo) {
+            if (wide) *reinterpret_cast<u32x4*>(gbase + 16u * (unsigned)at) = pack<DT>(v);
+            else {
+#pragma unroll
+                for (int e = 0; e < VEC<DT>; ++e) g0[at * VEC<DT> - sp.shift + e] = (elem_t<DT>)v[e];
+            }
+        }
+    }
+    if (edge >= 0) {
+        float v[VEC<DT>] = {ze};
+        rest_grad<DT>(v, s, c2);
+        g0[edge] = (elem_t<DT>)v[0];
+    }
+}
+template <int DT>
+__device__ __forceinline__ void store_zero(char* grow, const Span<DT>& sp, int t, int step, int c_hi, int edge) {
+    const bool wide = shift_of<DT>(grow) == sp.shift;
+    elem_t<DT>* g0 = reinterpret_cast<elem_t<DT>*>(grow);
+    char* gbase = grow - ((uintptr_t)grow & 15);
+    for (int at = t; at < c_hi; at += step) {
+        if (at < sp.c_lo) continue;
+        if (wide) *reinterpret_cast<u32x4*>(gbase + 16u * (unsigned)at) = u32x4{0u, 0u, 0u, 0u};
+        else {
+#pragma unroll
+            for (int e = 0; e < VEC<DT>; ++e) g0[at * VEC<DT> - sp.shift + e] = (elem_t<DT>)0.f;
+        }
+    }
+    if (edge >= 0) g0[edge] = (elem_t<DT>)0.f;
+}
+
+// One workgroup per row, the row in registers, C chunks a thread (T C 16 bytes of it): one read, one write.
 template <int DT, int T, int C>
 __global__ __launch_bounds__(T) void distill_row_kernel(const DistillArgs A) {
     static_assert(T >= ELG_TOP_MAX_K, "one entry per thread");
-    constexpr int W = T / 64, BITS = C ? T * C * VEC<DT> : SEG;
-    __shared__ unsigned bits[BITS / 32];
-    __shared__ int eidx[ELG_TOP_MAX_K];
-    __shared__ float eq[ELG_TOP_MAX_K];
-    __shared__ float fred[2 * 2 * W];
+    constexpr int W = T / 64;
+    __shared__ unsigned bits[T * C * VEC<DT> / 32];
+    __shared__ __attribute__((aligned(16))) int eidx[ELG_TOP_MAX_K];
+    __shared__ float ee[ELG_TOP_MAX_K];
+    __shared__ float mred[2 * W * 3], sred[2 * W * 4];
     const int tid = threadIdx.x, V = A.V, k = A.k;
-    BlockRed<W> red(fred);
+    BlockN<W, 3> bmax(mred);
+    BlockN<W, 4> bsum(sred);
     double lacc = 0.0;
+    for (int i = tid; i < T * C * VEC<DT> / 32; i += T) bits[i] = 0u;
+    if (tid < ELG_TOP_MAX_K) eidx[tid] = -2;
+    __syncthreads();
     for (long long r = blockIdx.x; r < A.R; r += gridDim.x) {
         const char* row = A.z + r * A.z_stride;
         char* grow = A.grad ? A.grad + r * A.g_stride : nullptr;
-        const int shift = shift_of<DT>(row), nch = (shift + V + VEC<DT> - 1) / VEC<DT>;
+        const Span<DT> sp(row, V);
         const float w = A.weight ? A.weight[r] : 1.f;
-        // ---- entries
-        int ei = -1;
-        float et = ELG_NEG_INF, zi = ELG_NEG_INF;
-        if (w != 0.f && tid < k) {
-            const long long i = index_any(A.ti, r * k + tid, A.ti_wide);
-            if (i >= 0 && i < V) {
-                ei = (int)i;
-                et = elem_any(A.tv, r * k + tid, A.tv_type);
-                zi = elem<DT>(row, i);
-            }
-        }
-        u32x4 zr[C ? C : 1];
-        if (C && w != 0.f) {
-#pragma unroll
-            for (int c = 0; c < C; ++c)
-                zr[c] = tid + c * T < nch ? load_chunk<DT>(row, shift, V, tid + c * T, PAD_NEG_INF<DT>) : u32x4{PAD_NEG_INF<DT>, PAD_NEG_INF<DT>, PAD_NEG_INF<DT>, PAD_NEG_INF<DT>};
-        }
+        const int edge = sp.edge(tid);
         if (w == 0.f) {                   // the row is not looked at
             if (tid == 0 && A.loss_rows) A.loss_rows[r] = 0.f;
-            if (grow) {
-                const float zero[VEC<DT>] = {};
-                for (int c = tid; c < nch; c += T) store_chunk<DT>(grow, shift, V, c, zero);
-            }
+            if (grow) store_zero<DT>(grow, sp, tid, T, sp.c_hi, edge);
             continue;
         }
-        if (tid < k) eidx[tid] = ei;
-        const float2 mx = red.max2(et, zi);
-        const float tm = mx.x > ELG_NEG_INF ? mx.x : 0.f, m_top = mx.y > ELG_NEG_INF ? mx.y : 0.f;
-        const float ee = ei >= 0 ? ex2((et - tm) * A.c2) : 0.f;
-        // first entry of its node?  (k broadcast reads; equal nodes are counted once in the softmax)
-        bool first = ei >= 0;
-        if (tid < k)
-            for (int j = 0; j < tid; ++j) first = first && eidx[j] != ei;
-        const float2 sm = red.sum2(ee, first ? ex2((zi - m_top) * A.c2) : 0.f);
-        const float st = sm.x, s_top = sm.y;
-        float a = A.tail ? A.tail[r] : 0.f;
-        a = a > 1.f ? 1.f : a < 0.f ? 0.f : a;
-        const float q = ei >= 0 && ee > 0.f ? ee * ((1.f - a) / st) : 0.f * ee;
-        if (tid < k) eq[tid] = q;
-        // ---- the rest: maximum and sum over the nodes of no entry
-        float rm = ELG_NEG_INF, rs = 0.f;
-        if (C) {
-            for (int i = tid; i < (nch * VEC<DT> + 31) / 32; i += T) bits[i] = 0u;
-            __syncthreads();
-            if (ei >= 0) atomicOr(bits + ((ei + shift) >> 5), 1u << ((ei + shift) & 31));
-            __syncthreads();
+        Entry en;
+        en.load(A, r);
+        // (what each pass needs of a chunk's place is formed there: kept from pass to pass it would not leave room for the row)
+        auto place = [&]() { int t = tid; asm volatile("" : "+v"(t)); return t; };
+        u32x4 zr[C];
+        const int t0 = place();
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const int pos = (tid + c * T) * VEC<DT>;
-                const unsigned b = tid + c * T < nch ? bits[pos >> 5] >> (pos & 31) : 0u;
-                float v[VEC<DT>];
-                unpack<DT>(zr[c], v);
-#pragma unroll
-                for (int e = 0; e < VEC<DT>; ++e) rm = fmaxf(rm, (b >> e) & 1u ? ELG_NEG_INF : v[e]);
-            }
-            rm = red.max2(rm, rm).x;
-            const float ref = rm > ELG_NEG_INF ? rm : 0.f;
-#pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const int pos = (tid + c * T) * VEC<DT>;
-                const unsigned b = tid + c * T < nch ? bits[pos >> 5] >> (pos & 31) : 0u;
-                float v[VEC<DT>];
-                unpack<DT>(zr[c], v);
-#pragma unroll
-                for (int e = 0; e < VEC<DT>; ++e) rs += (b >> e) & 1u ? 0.f : ex2((v[e] - ref) * A.c2);
-            }
-        } else {
-            for (int s0 = 0; s0 < nch * VEC<DT>; s0 += SEG) {
-                const int s1 = min(s0 + SEG, nch * VEC<DT>);
-                __syncthreads();
-                for (int i = tid; i < SEG / 32; i += T) bits[i] = 0u;
-                __syncthreads();
-                if (ei >= 0 && ei + shift >= s0 && ei + shift < s1) atomicOr(bits + ((ei + shift - s0) >> 5), 1u << ((ei + shift) & 31));
-                __syncthreads();
-                for (int c = s0 / VEC<DT> + tid; c < s1 / VEC<DT>; c += T) {
-                    const int pos = c * VEC<DT> - s0;
-                    const unsigned b = bits[pos >> 5] >> (pos & 31);
-                    float v[VEC<DT>], cm = ELG_NEG_INF;
-                    unpack<DT>(load_chunk<DT>(row, shift, V, c, PAD_NEG_INF<DT>), v);
-#pragma unroll
-                    for (int e = 0; e < VEC<DT>; ++e) {
-                        v[e] = (b >> e) & 1u ? ELG_NEG_INF : v[e];
-                        cm = fmaxf(cm, v[e]);
-                    }
-                    if (cm > rm) {
-                        rs = rm > ELG_NEG_INF ? rs * ex2((rm - cm) * A.c2) : rs;
-                        rm = cm;
-                    }
-                    const float ref = rm > ELG_NEG_INF ? rm : 0.f;
-#pragma unroll
-                    for (int e = 0; e < VEC<DT>; ++e) rs += ex2((v[e] - ref) * A.c2);
-                }
-            }
-            const float all = red.max2(rm, rm).x;
-            rs = rm > ELG_NEG_INF ? rs * ex2((rm - all) * A.c2) : rs;
-            rm = all;
+        for (int c = 0; c < C; ++c) {
+            constexpr unsigned pad = PAD_NEG_INF<DT>;
+            zr[c] = u32x4{pad, pad, pad, pad};
+            if (t0 >= sp.c_lo - c * T && t0 < sp.c_hi - c * T) zr[c] = sp.chunk(t0 + c * T);
         }
-        // ---- the row's scalars and its loss
-        const float m_rest = rm > ELG_NEG_INF ? rm : 0.f;
-        const float m = fmaxf(mx.y, rm);
-        const float f_top = mx.y > ELG_NEG_INF ? ex2((m_top - m) * A.c2) : 0.f, f_rest = rm > ELG_NEG_INF ? ex2((m_rest - m) * A.c2) : 0.f;
-        const float part_loss = q > 0.f || q != q ? q * (((et - tm) - (zi - m)) / A.tau) : 0.f;
-        const float2 lr = red.sum2(rs, part_loss);
-        const float s_rest = lr.x;
-        const float S = s_top * f_top + s_rest * f_rest;
-        const bool live = !(S <= 0.f) && !(st <= 0.f);
-        const float logS = logf(S);
+        float ze = edge >= 0 ? elem<DT>(row, edge) : ELG_NEG_INF;
+        if (tid < k) eidx[tid] = en.i;
+        if (en.i >= 0) atomicOr(bits + ((en.i + sp.shift) >> 5), 1u << ((en.i + sp.shift) & 31));
+        __syncthreads();
+        en.gather<DT>(row);
+        bool first, only;
+        en.twins(eidx, k, first, only);
+        // ---- the rest's maximum and sum, as the chunks arrive
+        Rest rest;
+        const int t1 = place();
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int pos = (t1 + c * T) * VEC<DT>;
+            float v[VEC<DT>];
+            unpack<DT>(zr[c], v);
+            hide_entries<DT>(v, bits[pos >> 5] >> (pos & 31));
+            rest.add(v, A.c2);
+        }
+        if (edge >= 0) {
+            const float v[1] = {bits[(edge + sp.shift) >> 5] >> ((edge + sp.shift) & 31) & 1u ? ELG_NEG_INF : ze};
+            rest.add(v, A.c2);
+        }
+        float mx[3] = {en.t, en.z, rest.m};
+        bmax.template run<true>(mx);
+        const float tm = mx[0] > ELG_NEG_INF ? mx[0] : 0.f, zm = mx[1] > ELG_NEG_INF ? mx[1] : 0.f, m = fmaxf(mx[1], mx[2]);
+        const float mine = en.i >= 0 ? ex2((en.t - tm) * A.c2) : 0.f;
+        float sm[4] = {mine, first ? ex2((en.z - zm) * A.c2) : 0.f, rest.to(mx[2], A.c2),
+                       mine > 0.f || mine != mine ? mine * ((en.t - tm) - (en.z - m)) : 0.f};
+        if (tid < k) ee[tid] = mine;
+        if (en.i >= 0) bits[(en.i + sp.shift) >> 5] = 0u;              // clean for the next row
+        bsum.template run<false>(sm);
+        const RowScalars s(A, r, w, mx[0], mx[1], mx[2], sm[0], sm[1], sm[2], sm[3]);
         if (tid == 0) {
-            float L = 0.f;
-            if (live) {
-                L = lr.y;
-                if (a < 1.f) L += (1.f - a) * (logf((1.f - a) / st) + logS);
-                if (a > 0.f) L += a * (logf(a) - ((m_rest - m) / A.tau + logf(s_rest) - logS));
-                L *= A.tau * A.tau * w;
-            }
-            if (A.loss_rows) A.loss_rows[r] = L * A.scale;
-            lacc += (double)L;
+            if (A.loss_rows) A.loss_rows[r] = s.loss * A.scale;
+            lacc += (double)s.loss;
         }
-        // ---- gradient: every node as one of the rest first, then the entries' nodes on top of it
         if (grow) {
-            const float cot = A.cot ? A.cot[r * A.cot_stride] : 1.f;
-            const float G = live ? A.scale * cot * w * A.tau : 0.f;
-            const float c_rest = live ? G * (f_rest / S - (a > 0.f && s_rest > 0.f ? a / s_rest : 0.f)) : 0.f;
-            if (C) {
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    if (tid + c * T >= nch) break;
-                    float v[VEC<DT>];
-                    unpack<DT>(zr[c], v);
-#pragma unroll
-                    for (int e = 0; e < VEC<DT>; ++e) v[e] = live ? ex2((v[e] - m_rest) * A.c2) * c_rest : 0.f;
-                    store_chunk<DT>(grow, shift, V, tid + c * T, v);
-                }
-            } else {
-                for (int c = tid; c < nch; c += T) {
-                    float v[VEC<DT>];
-                    unpack<DT>(load_chunk<DT>(row, shift, V, c, PAD_NEG_INF<DT>), v);
-#pragma unroll
-                    for (int e = 0; e < VEC<DT>; ++e) v[e] = live ? ex2((v[e] - m_rest) * A.c2) * c_rest : 0.f;
-                    store_chunk<DT>(grow, shift, V, c, v);
-                }
-            }
+            store_rest<DT, C>(grow, sp, place(), T, sp.c_hi, zr, edge, ze, s, A.c2);
             __syncthreads();
-            if (first && live) {
-                float qn = 0.f;
-                for (int j = 0; j < k; ++j) qn += eidx[j] == ei ? eq[j] : 0.f;
-                reinterpret_cast<elem_t<DT>*>(grow)[ei] = (elem_t<DT>)(G * (ex2((zi - m) * A.c2) / S - qn));
-            }
+            if (first && s.live) entry_grad<DT>(grow, en, eidx, ee, k, only, s, A.c2, mine);
         }
         __syncthreads();                  // the entries' LDS is written again by the next row
     }
     if (A.part && tid == 0) A.part[blockIdx.x] = lacc;
+}
+
+// Few long rows, or rows beyond what a workgroup can hold: a row is split into segments of SEG_T SEG_C chunks, a workgroup each.  The first
+// kernel leaves every segment's maximum and sum, the second joins them and writes the segments' gradients.
+constexpr int SEG_T = 256, SEG_C = 4;
+
+template <int DT>
+__device__ __forceinline__ void load_segment(u32x4 (&zr)[SEG_C], const Span<DT>& sp, int c0) {
+#pragma unroll
+    for (int c = 0; c < SEG_C; ++c) {
+        constexpr unsigned pad = PAD_NEG_INF<DT>;
+        const int at = c0 + c * SEG_T;
+        zr[c] = u32x4{pad, pad, pad, pad};
+        if (at >= sp.c_lo && at < sp.c_hi) zr[c] = sp.chunk(at);
+    }
+}
+
+template <int DT>
+__global__ __launch_bounds__(SEG_T) void distill_part_kernel(const DistillArgs A, float2* __restrict__ parts, int segs) {
+    constexpr int W = SEG_T / 64, POS = SEG_T * SEG_C * VEC<DT>;
+    __shared__ unsigned bits[POS / 32];
+    __shared__ unsigned edge_bits;
+    __shared__ float mred[2 * W], sred[2 * W];
+    const int tid = threadIdx.x, V = A.V;
+    const long long r = blockIdx.x / segs;
+    const int seg = (int)(blockIdx.x - r * segs), c_lo = seg * SEG_T * SEG_C;
+    const char* row = A.z + r * A.z_stride;
+    const Span<DT> sp(row, V);
+    if (A.weight && A.weight[r] == 0.f) return;
+    Entry en;
+    en.load(A, r);
+    u32x4 zr[SEG_C];
+    load_segment<DT>(zr, sp, c_lo + tid);
+    const int edge = seg == segs - 1 ? sp.edge(tid) : -1;             // the last segment takes the elements outside whole chunks
+    const float ze = edge >= 0 ? elem<DT>(row, edge) : ELG_NEG_INF;
+    for (int i = tid; i < POS / 32; i += SEG_T) bits[i] = 0u;
+    if (tid == 0) edge_bits = 0u;
+    __syncthreads();
+    const int p = en.i + sp.shift - c_lo * VEC<DT>;
+    if (en.i >= 0 && p >= 0 && p < POS) atomicOr(bits + (p >> 5), 1u << (p & 31));
+    if (en.i >= 0 && ((en.i + sp.shift) / VEC<DT> < sp.c_lo || (en.i + sp.shift) / VEC<DT> >= sp.c_hi)) atomicOr(&edge_bits, 1u << sp.edge_slot(en.i));
+    __syncthreads();
+    Rest rest;
+#pragma unroll
+    for (int c = 0; c < SEG_C; ++c) {
+        const int pos = (tid + c * SEG_T) * VEC<DT>;
+        float v[VEC<DT>];
+        unpack<DT>(zr[c], v);
+        hide_entries<DT>(v, bits[pos >> 5] >> (pos & 31));
+        rest.add(v, A.c2);
+    }
+    if (edge >= 0) {
+        const float v[1] = {edge_bits >> tid & 1u ? ELG_NEG_INF : ze};
+        rest.add(v, A.c2);
+    }
+    BlockN<W, 1> bmax(mred), bsum(sred);
+    float m[1] = {rest.m};
+    bmax.template run<true>(m);
+    float s[1] = {rest.to(m[0], A.c2)};
+    bsum.template run<false>(s);
+    if (tid == 0) parts[blockIdx.x] = make_float2(m[0], s[0]);
+}
+
+template <int DT>
+__global__ __launch_bounds__(SEG_T) void distill_join_kernel(const DistillArgs A, const float2* __restrict__ parts, int segs, int grid_segs) {
+    constexpr int W = SEG_T / 64;
+    __shared__ __attribute__((aligned(16))) int eidx[ELG_TOP_MAX_K];
+    __shared__ float ee[ELG_TOP_MAX_K];
+    __shared__ float mred[2 * W * 3], sred[2 * W * 4];
+    const int tid = threadIdx.x, V = A.V, k = A.k;
+    const long long r = blockIdx.x / grid_segs;
+    const int seg = (int)(blockIdx.x - r * grid_segs), c_lo = seg * SEG_T * SEG_C;
+    const char* row = A.z + r * A.z_stride;
+    char* grow = A.grad ? A.grad + r * A.g_stride : nullptr;
+    const Span<DT> sp(row, V);
+    const int c_end = min(sp.c_hi, c_lo + SEG_T * SEG_C), edge = seg == grid_segs - 1 ? sp.edge(tid) : -1;
+    const float w = A.weight ? A.weight[r] : 1.f;
+    if (w == 0.f) {
+        if (tid == 0 && seg == 0) {
+            if (A.loss_rows) A.loss_rows[r] = 0.f;
+            if (A.part) A.part[r] = 0.0;
+        }
+        if (grow) store_zero<DT>(grow, sp, c_lo + tid, SEG_T, c_end, edge);
+        return;
+    }
+    Entry en;
+    en.load(A, r);
+    Rest rest;                            // of the segments this thread joins
+    for (int i = tid; i < segs; i += SEG_T) {
+        const float2 p = parts[r * segs + i];
+        const float all = fmaxf(rest.m, p.x);
+        const float ref = all > ELG_NEG_INF ? all : 0.f;
+        rest.s = (rest.m > ELG_NEG_INF ? rest.s * ex2((rest.m - ref) * A.c2) : rest.s) + (p.x > ELG_NEG_INF ? p.y * ex2((p.x - ref) * A.c2) : p.y);
+        rest.m = all;
+    }
+    u32x4 zr[SEG_C];
+    if (grow) load_segment<DT>(zr, sp, c_lo + tid);
+    const float ze = grow && edge >= 0 ? elem<DT>(row, edge) : ELG_NEG_INF;
+    if (tid < ELG_TOP_MAX_K) eidx[tid] = tid < k ? en.i : -2;
+    en.gather<DT>(row);
+    float mx[3] = {en.t, en.z, rest.m};
+    BlockN<W, 3> bmax(mred);
+    BlockN<W, 4> bsum(sred);
+    bmax.template run<true>(mx);
+    bool first, only;
+    en.twins(eidx, k, first, only);
+    const float tm = mx[0] > ELG_NEG_INF ? mx[0] : 0.f, zm = mx[1] > ELG_NEG_INF ? mx[1] : 0.f, m = fmaxf(mx[1], mx[2]);
+    const float mine = en.i >= 0 ? ex2((en.t - tm) * A.c2) : 0.f;
+    float sm[4] = {mine, first ? ex2((en.z - zm) * A.c2) : 0.f, rest.to(mx[2], A.c2),
+                   mine > 0.f || mine != mine ? mine * ((en.t - tm) - (en.z - m)) : 0.f};
+    if (tid < k) ee[tid] = mine;
+    bsum.template run<false>(sm);
+    const RowScalars s(A, r, w, mx[0], mx[1], mx[2], sm[0], sm[1], sm[2], sm[3]);
+    if (tid == 0 && seg == 0) {
+        if (A.loss_rows) A.loss_rows[r] = s.loss * A.scale;
+        if (A.part) A.part[r] = (double)s.loss;
+    }
+    if (!grow) return;
+    store_rest<DT, SEG_C>(grow, sp, c_lo + tid, SEG_T, c_end, zr, edge, ze, s, A.c2);
+    __syncthreads();
+    // an entry's gradient is written by the workgroup that has written its node
+    const int c_of = (en.i + sp.shift) / VEC<DT>;
+    const bool whole = c_of >= sp.c_lo && c_of < sp.c_hi;
+    if (first && s.live && (whole ? c_of >= c_lo && c_of < c_end : seg == grid_segs - 1)) entry_grad<DT>(grow, en, eidx, ee, k, only, s, A.c2, mine);
 }
 
 // Short rows, G lanes per row (16: four rows to a wave; 64: one).  Lane l holds the nodes n = i G + l, i < NE, and the entries
@@ -421,13 +625,36 @@ void launch_small(const DistillArgs& A, int grid, hipStream_t s) {
     else hipLaunchKernelGGL((distill_small_kernel<DT, G, NE, KE, false>), dim3((unsigned)grid), dim3(256), 0, s, A);
 }
 
-// Rows of up to 256 logits take a quarter of a wave, up to 2048 a wave, longer ones a workgroup; the registers of a lane are sized by the
-// next power of two.
+// How a call is laid out, from its sizes alone (the scratch it needs follows from them too).
+struct Plan {
+    bool split;
+    int segs;
+    long long parts;                      // partial losses
+    Plan(long long R, long long V, int type) {
+        const int vec = type == ELG_F32 ? 4 : 8;
+        // rows that no workgroup can hold, or so few long ones that most of the chip would idle: measured, 6 rows of 100003 f32: 142 us a
+        // workgroup each, 24 us split; 256 rows of 32000 bf16: 16 and 19 us
+        split = V > 2048 && (V > 1024 * 16 * vec || (R <= 64 && V > 1024 * vec));
+        segs = split ? (int)((V + vec - 1 + SEG_T * SEG_C * vec - 1) / (SEG_T * SEG_C * vec)) : 0;     // a row may start inside its first 16 bytes
+        const long long rows_wg = V <= 256 ? 16 : V <= 2048 ? 4 : 1, want = (R + rows_wg - 1) / rows_wg;
+        parts = split ? R : want < MAX_GRID ? want : MAX_GRID;
+    }
+    long long bytes(long long R) const { return 8 * parts + 8 * R * segs; }
+};
+
+template <int DT, int T, int C>
+void launch_row(const DistillArgs& A, int grid, hipStream_t s) {
+    hipLaunchKernelGGL((distill_row_kernel<DT, T, C>), dim3((unsigned)grid), dim3(T), 0, s, A);
+}
+
+// Rows of up to 256 logits take a quarter of a wave, up to 2048 a wave (the registers of a lane sized by the next power of two), longer ones a
+// workgroup or several.
 template <int DT>
-int launch(const DistillArgs& A, hipStream_t s) {
-    const int V = A.V, k = A.k;
-    const long long rows_wg = V <= 256 ? 16 : V <= 2048 ? 4 : 1, want = (A.R + rows_wg - 1) / rows_wg;
-    const int grid = (int)(want < MAX_GRID ? want : MAX_GRID);
+void launch(const DistillArgs& A, const Plan& P, float2* parts, hipStream_t s) {
+    const int V = A.V, k = A.k, grid = (int)P.parts;
+    // chunks a row can span: its own and, unless every row starts on 16 bytes, what the first line holds in front of it
+    const bool aligned = !((uintptr_t)A.z & 15) && !(A.z_stride & 15);
+    const int nch = (V + (aligned ? 0 : VEC<DT> - 1) + VEC<DT> - 1) / VEC<DT>;
     if (V <= 256) {
         if (k > 48) V <= 128 ? launch_small<DT, 16, 8, 16>(A, grid, s) : launch_small<DT, 16, 16, 16>(A, grid, s);
         else if (k > 16) V <= 64 ? launch_small<DT, 16, 4, 3>(A, grid, s) : V <= 128 ? launch_small<DT, 16, 8, 3>(A, grid, s) : launch_small<DT, 16, 16, 3>(A, grid, s);
@@ -436,8 +663,16 @@ int launch(const DistillArgs& A, hipStream_t s) {
     } else if (V <= 2048) {
         if (k <= 64) V <= 512 ? launch_small<DT, 64, 8, 1>(A, grid, s) : V <= 1024 ? launch_small<DT, 64, 16, 1>(A, grid, s) : launch_small<DT, 64, 32, 1>(A, grid, s);
         else V <= 512 ? launch_small<DT, 64, 8, 4>(A, grid, s) : V <= 1024 ? launch_small<DT, 64, 16, 4>(A, grid, s) : launch_small<DT, 64, 32, 4>(A, grid, s);
-    } else hipLaunchKernelGGL((distill_row_kernel<DT, 256, 0>), dim3((unsigned)grid), dim3(256), 0, s, A);
-    return grid;
+    } else if (P.split) {
+        const int grad_segs = A.grad ? P.segs : 1;
+        hipLaunchKernelGGL((distill_part_kernel<DT>), dim3((unsigned)(A.R * P.segs)), dim3(SEG_T), 0, s, A, parts, P.segs);
+        hipLaunchKernelGGL((distill_join_kernel<DT>), dim3((unsigned)(A.R * grad_segs)), dim3(SEG_T), 0, s, A, parts, P.segs, grad_segs);
+    } else if (nch <= 256 * 4) launch_row<DT, 256, 4>(A, grid, s);
+    else if (nch <= 256 * 8) launch_row<DT, 256, 8>(A, grid, s);
+    else if (nch <= 512 * 8) launch_row<DT, 512, 8>(A, grid, s);
+    else if (nch <= 1024 * 8) launch_row<DT, 1024, 8>(A, grid, s);
+    else if (nch <= 1024 * 16) launch_row<DT, 1024, 16>(A, grid, s);
+    else launch_row<DT, 1024, 17>(A, grid, s);
 }
 
 }  // namespace
@@ -446,8 +681,8 @@ int launch(const DistillArgs& A, hipStream_t s) {
 using namespace elg;
 
 extern "C" int64_t elg_distill_ws_bytes(int64_t R, int64_t V, int type) {
-    (void)V; (void)type;
-    return 8 * (R < MAX_GRID ? (R > 0 ? R : 1) : MAX_GRID);
+    if (R <= 0 || V <= 0 || V > ELG_ROW_MAX_V) return 0;
+    return Plan(R, V, type).bytes(R);
 }
 
 extern "C" int elg_distill_loss_grad(const void* z, int64_t z_stride, int type, int64_t R, int64_t V, const void* top_values, int top_type,
@@ -462,7 +697,9 @@ extern "C" int elg_distill_loss_grad(const void* z, int64_t z_stride, int type, 
     if (cot_stride != 0 && cot_stride != 1) return fail(ELG_EINVAL, "distill: the cotangent is one number or one per row");
     if (!loss_rows && !loss_total && !grad) return fail(ELG_EINVAL, "distill: nothing to compute");
     if (R > 0 && (!z || !top_values || !top_idx)) return fail(ELG_EINVAL, "distill: null buffer");
-    if (loss_total && (!ws || ws_bytes < elg_distill_ws_bytes(R, V, type))) return fail(ELG_EINVAL, "distill: loss_total needs elg_distill_ws_bytes() of scratch");
+    const Plan P(R, V, type);
+    if (R > 0 && (loss_total || P.split) && (!ws || ws_bytes < P.bytes(R))) return fail(ELG_EINVAL, "distill: needs elg_distill_ws_bytes() of scratch");
+    if (R * (P.segs + 1) > 0x7FFFFFFF) return fail(ELG_EINVAL, "distill: too many long rows for one call");
     if (R == 0 && !loss_total) return ELG_OK;
     const int es = type == ELG_F32 ? 4 : 2;
     if (((uintptr_t)z | (uintptr_t)grad) % es || (uintptr_t)top_values % (top_type == ELG_F32 ? 4 : 2) || (uintptr_t)top_idx % (idx_wide ? 8 : 4) || (uintptr_t)ws % 8)
@@ -475,11 +712,11 @@ extern "C" int elg_distill_loss_grad(const void* z, int64_t z_stride, int type, 
     A.loss_rows = loss_rows; A.part = loss_total ? (double*)ws : nullptr;
     A.grad = (char*)grad; A.g_stride = V * es;
     (void)hipGetLastError();
-    int G = 0;
+    hipStream_t st = (hipStream_t)stream;
     if (R > 0) {
-        hipStream_t st = (hipStream_t)stream;
-        G = type == ELG_F32 ? launch<ELG_F32>(A, st) : type == ELG_BF16 ? launch<ELG_BF16>(A, st) : launch<ELG_F16>(A, st);
+        float2* parts = reinterpret_cast<float2*>((char*)ws + 8 * P.parts);
+        type == ELG_F32 ? launch<ELG_F32>(A, P, parts, st) : type == ELG_BF16 ? launch<ELG_BF16>(A, P, parts, st) : launch<ELG_F16>(A, P, parts, st);
     }
-    if (loss_total) hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, (const double*)ws, G, scale, loss_total);
+    if (loss_total) hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(256), 0, st, (const double*)ws, R > 0 ? (int)P.parts : 0, scale, loss_total);
     return launch_status("distill");
 }

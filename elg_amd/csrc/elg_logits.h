@@ -116,6 +116,31 @@ __device__ __forceinline__ void store_chunk(void* row, int shift, int V, int c, 
     }
 }
 
+// The same row as whole chunks [c_lo, c_hi) and the few elements in front of and behind them: loops over whole chunks need no per-chunk
+// case distinction, and thread t < 2 VEC takes the single element edge(t) besides.  For rows of at least 2 VEC elements.
+template <int DT>
+struct Span {
+    const char* base;                     // 16-byte aligned; chunk c is at base + 16 c
+    int shift, c_lo, c_hi, V;
+    __device__ __forceinline__ Span(const void* row, int V_) : V(V_) {
+        shift = shift_of<DT>(row);
+        base = reinterpret_cast<const char*>(row) - ((uintptr_t)row & 15);
+        c_lo = shift ? 1 : 0;
+        c_hi = (shift + V) / VEC<DT>;
+    }
+    __device__ __forceinline__ int edge(int t) const {
+        const int head = shift ? VEC<DT> - shift : 0, tail = c_hi * VEC<DT> - shift;
+        const int n = t < head ? t : tail + t - head;
+        return n < V && t < 2 * VEC<DT> ? n : -1;
+    }
+    // the thread whose edge element is n (n outside the whole chunks)
+    __device__ __forceinline__ int edge_slot(int n) const {
+        const int head = shift ? VEC<DT> - shift : 0;
+        return n < head ? n : head + n - (c_hi * VEC<DT> - shift);
+    }
+    __device__ __forceinline__ u32x4 chunk(int c) const { return *reinterpret_cast<const u32x4*>(base + 16u * (unsigned)c); }
+};
+
 // block-wide sum / max: one LDS exchange and one barrier each; `slot` alternates between two buffers so that a wave may enter the next
 // reduction while another still reads this one.  Every thread gets the result, added in wave order (the same bits in every run).
 template <int W>

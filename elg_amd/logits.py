@@ -113,7 +113,7 @@ class _Teacher:
         R, V = z.shape
         ws, n = None, 0
         lib = L.lib()
-        if total is not None:
+        if total is not None or V > 2048:
             n = lib.elg_distill_ws_bytes(R, V, self.type)
             ws = torch.empty(n, dtype=torch.uint8, device=z.device)
         L.check(lib.elg_distill_loss_grad(_p(z), z.stride(0), self.type, R, V, _p(self.values), self.top_type, _p(self.idx),
@@ -243,7 +243,11 @@ def verify_draft(target_probs: torch.Tensor, draft_tokens: torch.Tensor, uniform
         lengths = lengths.to(torch.int32).contiguous()
     tokens = torch.empty(*lead, G + 1, dtype=torch.int32, device=p.device)
     accepted = torch.empty(lead, dtype=torch.int32, device=p.device)
-    L.check(L.lib().elg_verify_draft(_p(p), p.stride(0), p.stride(1), _p(q), q.stride(0) if q is not None else 0,
+    lib, ws, n = L.lib(), None, 0
+    if V > 1024:
+        n = lib.elg_verify_ws_bytes(B, V, ty)
+        ws = torch.empty(n, dtype=torch.uint8, device=p.device) if n else None
+    L.check(lib.elg_verify_draft(_p(p), p.stride(0), p.stride(1), _p(q), q.stride(0) if q is not None else 0,
                                      q.stride(1) if q is not None else 0, ty, _p(x), int(x.dtype == torch.int64), G, _p(u), G + 1,
-                                     _p(lengths), B, G, V, _p(tokens), _p(accepted), _stream()), "elg_verify_draft")
+                                     _p(lengths), B, G, V, _p(tokens), _p(accepted), _p(ws), n, _stream()), "elg_verify_draft")
     return tokens, accepted

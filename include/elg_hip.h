@@ -494,9 +494,9 @@ int elg_top_logits(const void* z, int64_t z_stride, int type, int64_t R, int64_t
  * tail (R) in [0, 1] or NULL (0), weight (R) or NULL (1).  A row of weight 0 is not read; it, a row without an open node and a row
  * without an entry above -inf have loss 0 and gradient 0.  A teacher probability on a node the student has closed makes the loss +inf.
  *   loss_rows (R) or NULL  = scale L_r
- *   loss_total (1) or NULL = scale sum_r L_r, added in 64 bits in an order of its own fixed by R (needs ws)
+ *   loss_total (1) or NULL = scale sum_r L_r, added in 64 bits in an order fixed by the sizes
  *   grad (R,V) packed, of `type`, or NULL = scale cot_r dL_r/dz; cot: NULL (1), one number (cot_stride 0) or one per row (1)
- * ws: elg_distill_ws_bytes() bytes, 8-byte aligned. */
+ * ws: elg_distill_ws_bytes() bytes, 8-byte aligned; may be NULL for rows of up to 2048 logits without loss_total. */
 int64_t elg_distill_ws_bytes(int64_t R, int64_t V, int type);
 int elg_distill_loss_grad(const void* z, int64_t z_stride, int type, int64_t R, int64_t V, const void* top_values, int top_type,
                           const void* top_idx, int idx_wide, int k, const float* tail, float temperature, const float* weight,
@@ -508,11 +508,13 @@ int elg_distill_loss_grad(const void* z, int64_t z_stride, int type, int64_t R, 
  * lengths (B) or NULL (G): drafts of each sequence.  Draft i is accepted while uniforms(b,i) q(x_i) < p(x_i); a token outside
  * [0, V) is refused.  accepted (B) = the drafts in front of the first refusal; out_tokens (B,G+1) = these, then the first n with
  * cumsum(r)_n > uniforms(b,G) sum(r), then -1; r = max(p - q, 0) at the refused draft, p where that is all zero or nothing was
- * refused, and -1 is drawn where p is zero too.  Rows need not sum to 1; entries that are not positive count as 0. */
+ * refused, and -1 is drawn where p is zero too.  Rows need not sum to 1; entries that are not positive count as 0.
+ * ws: elg_verify_ws_bytes() bytes, 16-byte aligned (0 bytes: may be NULL). */
+int64_t elg_verify_ws_bytes(int64_t B, int64_t V, int type);
 int elg_verify_draft(const void* target, int64_t target_bstride, int64_t target_sstride, const void* draft, int64_t draft_bstride,
                      int64_t draft_sstride, int type, const void* tokens, int tokens_wide, int64_t tokens_stride, const float* uniforms,
                      int64_t uniforms_stride, const int32_t* lengths, int64_t B, int G, int64_t V, int32_t* out_tokens,
-                     int32_t* accepted, void* stream);
+                     int32_t* accepted, void* ws, int64_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -307,10 +307,11 @@ def test_distill_writes_inside_its_rows_only(V):
     z = rows("plain", 5, V, 2)
     tv, ti, a = teacher_of(z, 9, 2)
     d = [t.to(DEV) for t in (z, tv, ti, a)]
+    ws = torch.empty(L.lib().elg_distill_ws_bytes(5, V, L.F32), dtype=torch.uint8, device=DEV)
     for off in (1, 2, 3, 64):
         buf = torch.full((off + 5 * V + 70,), 7.0, device=DEV)
         rc = L.lib().elg_distill_loss_grad(d[0].data_ptr(), V, L.F32, 5, V, d[1].data_ptr(), L.F32, d[2].data_ptr(), 0, 9, d[3].data_ptr(),
-                                           1.0, None, None, 0, 1.0, None, None, buf.data_ptr() + 4 * off, None, 0,
+                                           1.0, None, None, 0, 1.0, None, None, buf.data_ptr() + 4 * off, ws.data_ptr(), ws.numel(),
                                            torch.cuda.current_stream().cuda_stream)
         assert rc == 0
         _, ref = lg().distill_loss_grad(*d[:3], tail=d[3], reduction="none")

@@ -31,7 +31,7 @@ def distill(**o):
 
 def verify(**o):
     L, c = lib()
-    a = dict(p=P, pb=30, ps=10, q=None, qb=0, qs=0, type=0, x=P, wide=0, xs=2, u=P, us=3, n=None, B=4, G=2, V=10, out=P, acc=P, stream=None)
+    a = dict(p=P, pb=30, ps=10, q=None, qb=0, qs=0, type=0, x=P, wide=0, xs=2, u=P, us=3, n=None, B=4, G=2, V=10, out=P, acc=P, ws=None, n_ws=0, stream=None)
     a.update(o)
     return c.elg_verify_draft(*a.values())
 
@@ -42,11 +42,12 @@ def verify(**o):
     (top, dict(t=float("inf"))), (top, dict(z=None)), (top, dict(values=None)), (top, dict(idx=None)), (top, dict(z=P + 2)), (top, dict(values=P + 1)),
     (distill, dict(type=3)), (distill, dict(ttype=9)), (distill, dict(R=-1)), (distill, dict(V=0)), (distill, dict(V=1 << 33)), (distill, dict(k=0)),
     (distill, dict(k=257)), (distill, dict(t=0.0)), (distill, dict(t=float("inf"))), (distill, dict(cs=2)), (distill, dict(rows=None)),
-    (distill, dict(z=None)), (distill, dict(tv=None)), (distill, dict(ti=None)), (distill, dict(total=P)), (distill, dict(total=P, ws=P, n=8)),
+    (distill, dict(z=None)), (distill, dict(tv=None)), (distill, dict(ti=None)), (distill, dict(total=P)), (distill, dict(total=P, ws=P, n=7)),
     (distill, dict(total=P, ws=P + 4, n=1 << 20)), (distill, dict(grad=P + 1)), (distill, dict(z=P + 2)), (distill, dict(ti=P + 4, wide=1)),
     (verify, dict(type=7)), (verify, dict(B=-1)), (verify, dict(G=-1)), (verify, dict(G=1025)), (verify, dict(V=0)), (verify, dict(V=1 << 33)),
     (verify, dict(p=None)), (verify, dict(x=None)), (verify, dict(u=None)), (verify, dict(out=None)), (verify, dict(acc=None)), (verify, dict(p=P + 2)),
-    (verify, dict(x=P + 4, wide=1))])
+    (verify, dict(x=P + 4, wide=1)), (verify, dict(V=9000)), (verify, dict(V=9000, ws=P, n_ws=16)), (verify, dict(V=9000, ws=P + 8, n_ws=1 << 20)),
+    (distill, dict(V=9000)), (distill, dict(V=200000, R=1000, ws=P, n=64))])
 def test_refused_at_the_c_entry(call, bad):
     L, c = lib()
     assert call(**bad) == L.ELG_EINVAL
