@@ -31,6 +31,7 @@ struct DistillArgs {
     float scale;
     float* loss_rows;
     double* part;                         // one partial loss per workgroup, or null
+    float* total;                         // the loss itself, where one workgroup sees every row; or null
     char* grad;                           // (R, V) packed, or null
     long long g_stride;                   // bytes
 };
@@ -567,7 +568,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistillArgs A)
         const bool live = on && !(S <= 0.f) && !(st <= 0.f);
         const float inv_S = __builtin_amdgcn_rcpf(S);
         // ---- loss
-        if (A.loss_rows || A.part) {
+        if (A.loss_rows || A.part || A.total) {
             float L = 0.f;
 #pragma unroll
             for (int e = 0; e < KE; ++e) L += q[e] > 0.f || q[e] != q[e] ? q[e] * ((et[e] - tm) - (zi[e] - m)) : 0.f;
@@ -594,12 +595,16 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistillArgs A)
             }
         }
     }
-    if (A.part) {
+    if (A.part || A.total) {
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) lacc += __shfl_xor(lacc, d, 64);
         if (lane == 0) dred[wave] = lacc;
         __syncthreads();
-        if (threadIdx.x == 0) A.part[blockIdx.x] = (dred[0] + dred[1]) + (dred[2] + dred[3]);
+        if (threadIdx.x == 0) {
+            const double all = (dred[0] + dred[1]) + (dred[2] + dred[3]);
+            if (A.total) A.total[0] = (float)(all * (double)A.scale);
+            else A.part[blockIdx.x] = all;
+        }
     }
 }
 
@@ -629,7 +634,8 @@ void launch_small(const DistillArgs& A, int grid, hipStream_t s) {
 struct Plan {
     bool split;
     int segs;
-    long long parts;                      // partial losses
+    bool one;                             // so few short rows that one workgroup forms their total: a launch and the scratch saved
+    long long parts;                      // workgroups and, unless `one`, partial losses
     Plan(long long R, long long V, int type) {
         const int vec = type == ELG_F32 ? 4 : 8;
         // rows that no workgroup can hold, or so few long ones that most of the chip would idle: measured, 6 rows of 100003 f32: 142 us a
@@ -637,9 +643,10 @@ struct Plan {
         split = V > 2048 && (V > 1024 * 16 * vec || (R <= 64 && V > 1024 * vec));
         segs = split ? (int)((V + vec - 1 + SEG_T * SEG_C * vec - 1) / (SEG_T * SEG_C * vec)) : 0;     // a row may start inside its first 16 bytes
         const long long rows_wg = V <= 256 ? 16 : V <= 2048 ? 4 : 1, want = (R + rows_wg - 1) / rows_wg;
+        one = V <= 2048 && want <= 8;
         parts = split ? R : want < MAX_GRID ? want : MAX_GRID;
     }
-    long long bytes(long long R) const { return 8 * parts + 8 * R * segs; }
+    long long bytes(long long R) const { return one ? 0 : 8 * parts + 8 * R * segs; }
 };
 
 template <int DT, int T, int C>
@@ -651,7 +658,7 @@ void launch_row(const DistillArgs& A, int grid, hipStream_t s) {
 // workgroup or several.
 template <int DT>
 void launch(const DistillArgs& A, const Plan& P, float2* parts, hipStream_t s) {
-    const int V = A.V, k = A.k, grid = (int)P.parts;
+    const int V = A.V, k = A.k, grid = A.total ? 1 : (int)P.parts;
     // chunks a row can span: its own and, unless every row starts on 16 bytes, what the first line holds in front of it
     const bool aligned = !((uintptr_t)A.z & 15) && !(A.z_stride & 15);
     const int nch = (V + (aligned ? 0 : VEC<DT> - 1) + VEC<DT> - 1) / VEC<DT>;
@@ -698,7 +705,7 @@ extern "C" int elg_distill_loss_grad(const void* z, int64_t z_stride, int type, 
     if (!loss_rows && !loss_total && !grad) return fail(ELG_EINVAL, "distill: nothing to compute");
     if (R > 0 && (!z || !top_values || !top_idx)) return fail(ELG_EINVAL, "distill: null buffer");
     const Plan P(R, V, type);
-    if (R > 0 && (loss_total || P.split) && (!ws || ws_bytes < P.bytes(R))) return fail(ELG_EINVAL, "distill: needs elg_distill_ws_bytes() of scratch");
+    if (R > 0 && P.bytes(R) > 0 && (loss_total || P.split) && (!ws || ws_bytes < P.bytes(R))) return fail(ELG_EINVAL, "distill: needs elg_distill_ws_bytes() of scratch");
     if (R * (P.segs + 1) > 0x7FFFFFFF) return fail(ELG_EINVAL, "distill: too many long rows for one call");
     if (R == 0 && !loss_total) return ELG_OK;
     const int es = type == ELG_F32 ? 4 : 2;
@@ -709,7 +716,7 @@ extern "C" int elg_distill_loss_grad(const void* z, int64_t z_stride, int type, 
     A.tv = top_values; A.ti = top_idx; A.tv_type = top_type; A.ti_wide = idx_wide != 0;
     A.tail = tail; A.weight = weight; A.cot = cot; A.cot_stride = cot_stride;
     A.tau = temperature; A.c2 = LOG2E / temperature; A.scale = scale;
-    A.loss_rows = loss_rows; A.part = loss_total ? (double*)ws : nullptr;
+    A.loss_rows = loss_rows; A.part = loss_total && !P.one ? (double*)ws : nullptr; A.total = P.one ? loss_total : nullptr;
     A.grad = (char*)grad; A.g_stride = V * es;
     (void)hipGetLastError();
     hipStream_t st = (hipStream_t)stream;
@@ -717,6 +724,6 @@ extern "C" int elg_distill_loss_grad(const void* z, int64_t z_stride, int type, 
         float2* parts = reinterpret_cast<float2*>((char*)ws + 8 * P.parts);
         type == ELG_F32 ? launch<ELG_F32>(A, P, parts, st) : type == ELG_BF16 ? launch<ELG_BF16>(A, P, parts, st) : launch<ELG_F16>(A, P, parts, st);
     }
-    if (loss_total) hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(256), 0, st, (const double*)ws, R > 0 ? (int)P.parts : 0, scale, loss_total);
+    if (loss_total && !(P.one && R > 0)) hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(256), 0, st, (const double*)ws, R > 0 ? (int)P.parts : 0, scale, loss_total);
     return launch_status("distill");
 }

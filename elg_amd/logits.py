@@ -11,6 +11,7 @@ Each is one call into libelg_hip.so (include/elg_hip.h) on the current stream, w
 live on the current device; rows may be strided views (the last dimension contiguous), others are copied."""
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -21,8 +22,19 @@ from .engine import _need_cuda
 _TYPES = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # a tenth of the time of current_stream()'s object
+
+
 def _stream() -> int:
+    """The current stream of the current device (which every input has been checked to live on)."""
+    if _raw_stream is not None:
+        return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+@functools.lru_cache(maxsize=256)
+def _distill_ws_bytes(R: int, V: int, ty: int) -> int:
+    return int(L.lib().elg_distill_ws_bytes(R, V, ty))
 
 
 def _p(t: Optional[torch.Tensor]):
@@ -114,8 +126,8 @@ class _Teacher:
         ws, n = None, 0
         lib = L.lib()
         if total is not None or V > 2048:
-            n = lib.elg_distill_ws_bytes(R, V, self.type)
-            ws = torch.empty(n, dtype=torch.uint8, device=z.device)
+            n = _distill_ws_bytes(R, V, self.type)
+            ws = torch.empty(n, dtype=torch.uint8, device=z.device) if n else None
         L.check(lib.elg_distill_loss_grad(_p(z), z.stride(0), self.type, R, V, _p(self.values), self.top_type, _p(self.idx),
                                           int(self.idx.dtype == torch.int64), self.k, _p(self.tail), self.temperature, _p(self.weight),
                                           _p(cot), cot_stride, scale, _p(rows), _p(total), _p(grad), _p(ws), n, _stream()),
@@ -147,14 +159,23 @@ class _DistillLoss(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gout):
+    def gradient(ctx, gout):
         logits = ctx.saved_tensors[0]
         z = _rows(logits, "logits")
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
         if z.shape[0]:
-            ctx.teacher.call(z, cot=gout.contiguous().float(), cot_stride=int(ctx.reduction == "none"), scale=ctx.scale, grad=grad)
+            if gout.dtype != torch.float32 or not gout.is_contiguous():
+                gout = gout.float().contiguous()
+            ctx.teacher.call(z, cot=gout, cot_stride=int(ctx.reduction == "none"), scale=ctx.scale, grad=grad)
         return (grad, None, None) + (None,) * (len(ctx.saved_tensors) - 1)
+
+    @staticmethod
+    def backward(ctx, gout):
+        # only a backward that builds a graph (create_graph=True) needs its outputs marked as differentiable no further
+        return _distill_gradient_once(ctx, gout) if torch.is_grad_enabled() else _DistillLoss.gradient(ctx, gout)
+
+
+_distill_gradient_once = torch.autograd.function.once_differentiable(_DistillLoss.gradient)
 
 
 def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_idx: torch.Tensor, *, tail: Optional[torch.Tensor] = None,

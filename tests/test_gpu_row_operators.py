@@ -536,6 +536,9 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             f()
     leaf = z.clone().requires_grad_(True)
+    (g,) = torch.autograd.grad(lg().distill_loss(leaf, v, i), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()                                 # once, not twice
     loss = lg().distill_loss(leaf, v, i)
     v.add_(1.0)                                            # the teacher was overwritten before the backward
     with pytest.raises(RuntimeError):

@@ -42,8 +42,8 @@ def verify(**o):
     (top, dict(t=float("inf"))), (top, dict(z=None)), (top, dict(values=None)), (top, dict(idx=None)), (top, dict(z=P + 2)), (top, dict(values=P + 1)),
     (distill, dict(type=3)), (distill, dict(ttype=9)), (distill, dict(R=-1)), (distill, dict(V=0)), (distill, dict(V=1 << 33)), (distill, dict(k=0)),
     (distill, dict(k=257)), (distill, dict(t=0.0)), (distill, dict(t=float("inf"))), (distill, dict(cs=2)), (distill, dict(rows=None)),
-    (distill, dict(z=None)), (distill, dict(tv=None)), (distill, dict(ti=None)), (distill, dict(total=P)), (distill, dict(total=P, ws=P, n=7)),
-    (distill, dict(total=P, ws=P + 4, n=1 << 20)), (distill, dict(grad=P + 1)), (distill, dict(z=P + 2)), (distill, dict(ti=P + 4, wide=1)),
+    (distill, dict(z=None)), (distill, dict(tv=None)), (distill, dict(ti=None)), (distill, dict(total=P, R=4000)), (distill, dict(total=P, R=400, ws=P, n=7)),
+    (distill, dict(total=P, R=400, ws=P + 4, n=1 << 20)), (distill, dict(grad=P + 1)), (distill, dict(z=P + 2)), (distill, dict(ti=P + 4, wide=1)),
     (verify, dict(type=7)), (verify, dict(B=-1)), (verify, dict(G=-1)), (verify, dict(G=1025)), (verify, dict(V=0)), (verify, dict(V=1 << 33)),
     (verify, dict(p=None)), (verify, dict(x=None)), (verify, dict(u=None)), (verify, dict(out=None)), (verify, dict(acc=None)), (verify, dict(p=P + 2)),
     (verify, dict(x=P + 4, wide=1)), (verify, dict(V=9000)), (verify, dict(V=9000, ws=P, n_ws=16)), (verify, dict(V=9000, ws=P + 8, n_ws=1 << 20)),
