@@ -42,11 +42,18 @@ def _p(t: Optional[torch.Tensor]):
 
 
 def _type(t: torch.Tensor, what: str) -> int:
+    """The element type of a call's first tensor, which must live on the current device."""
     _need_cuda(t, what)
     ty = _TYPES.get(t.dtype)
     if ty is None:
         raise ValueError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
     return ty
+
+
+def _beside(t: torch.Tensor, dev: int, what: str):
+    """Another tensor of the call: on the same device `dev`, which is the current one."""
+    if t.get_device() != dev:
+        _need_cuda(t, what)
 
 
 def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -65,10 +72,10 @@ def _temperature(t: float) -> float:
     return t
 
 
-def _per_row(t: Optional[torch.Tensor], lead, what: str) -> Optional[torch.Tensor]:
+def _per_row(t: Optional[torch.Tensor], lead, dev: int, what: str) -> Optional[torch.Tensor]:
     if t is None:
         return None
-    _need_cuda(t, what)
+    _beside(t, dev, what)
     if t.shape != lead:
         raise ValueError(f"{what} must hold one number per row: {tuple(lead)}, got {tuple(t.shape)}")
     if t.dtype != torch.float32:
@@ -83,15 +90,15 @@ def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0, with_t
     (-inf), lowest index first.  No gradient flows through (the teacher is a constant)."""
     ty = _type(logits, "logits")
     temperature = _temperature(temperature)
-    z = _rows(logits.detach(), "logits")
+    z = _rows(logits, "logits")
     R, V = z.shape
     k = int(k)
     if not 1 <= k <= min(V, L.TOP_MAX_K):
         raise ValueError(f"k must be 1 .. min(V, {L.TOP_MAX_K}), got k = {k} for rows of {V}")
     lead = logits.shape[:-1]
-    values = torch.empty(*lead, k, dtype=z.dtype, device=z.device)
-    idx = torch.empty(*lead, k, dtype=torch.int32, device=z.device)
-    tail = torch.empty(lead, dtype=torch.float32, device=z.device) if with_tail else None
+    values = z.new_empty((*lead, k))
+    idx = z.new_empty((*lead, k), dtype=torch.int32)
+    tail = z.new_empty(lead, dtype=torch.float32) if with_tail else None
     L.check(L.lib().elg_top_logits(_p(z), z.stride(0), ty, R, V, k, temperature, _p(values), _p(idx), _p(tail), _stream()),
             "elg_top_logits")
     return (values, idx, tail) if with_tail else (values, idx)
@@ -102,9 +109,13 @@ class _Teacher:
 
     def __init__(self, logits, values, idx, tail, temperature, weight):
         self.type = _type(logits, "logits")
-        self.top_type = _type(values, "top_values")
-        _need_cuda(idx, "top_idx")
-        if idx.dtype not in (torch.int32, torch.int64):
+        dev = logits.get_device()
+        _beside(values, dev, "top_values")
+        _beside(idx, dev, "top_idx")
+        self.top_type = _TYPES.get(values.dtype)
+        if self.top_type is None:
+            raise ValueError(f"top_values must be float32, bfloat16 or float16, got {values.dtype}")
+        if idx.dtype is not torch.int32 and idx.dtype is not torch.int64:
             raise ValueError(f"top_idx must be int32 or int64, got {idx.dtype}")
         lead = logits.shape[:-1]
         if values.shape != idx.shape or values.dim() == 0 or values.shape[:-1] != lead:
@@ -112,12 +123,12 @@ class _Teacher:
         self.k = values.shape[-1]
         if not 1 <= self.k <= L.TOP_MAX_K:
             raise ValueError(f"1 .. {L.TOP_MAX_K} teacher entries a row, got {self.k}")
-        if torch.is_grad_enabled() and (values.requires_grad or (tail is not None and tail.requires_grad)
-                                        or (weight is not None and weight.requires_grad)):
+        if (values.requires_grad or (tail is not None and tail.requires_grad) or (weight is not None and weight.requires_grad)) \
+                and torch.is_grad_enabled():
             raise ValueError("no gradient flows to the teacher's logits, the tail or the weights: detach them")
         self.values, self.idx = values.contiguous(), idx.contiguous()
-        self.tail = _per_row(tail, lead, "tail")
-        self.weight = _per_row(weight, lead, "weight")
+        self.tail = _per_row(tail, lead, dev, "tail")
+        self.weight = _per_row(weight, lead, dev, "weight")
         self.temperature = _temperature(temperature)
         self.lead = lead
 
@@ -127,7 +138,7 @@ class _Teacher:
         lib = L.lib()
         if total is not None or V > 2048:
             n = _distill_ws_bytes(R, V, self.type)
-            ws = torch.empty(n, dtype=torch.uint8, device=z.device) if n else None
+            ws = z.new_empty(n, dtype=torch.uint8) if n else None
         L.check(lib.elg_distill_loss_grad(_p(z), z.stride(0), self.type, R, V, _p(self.values), self.top_type, _p(self.idx),
                                           int(self.idx.dtype == torch.int64), self.k, _p(self.tail), self.temperature, _p(self.weight),
                                           _p(cot), cot_stride, scale, _p(rows), _p(total), _p(grad), _p(ws), n, _stream()),
@@ -150,11 +161,11 @@ class _DistillLoss(torch.autograd.Function):
         ctx.teacher, ctx.scale, ctx.reduction = teacher, scale, reduction
         ctx.save_for_backward(logits, *saved)        # the teacher's tensors too: writing to one before the backward is an error, not a wrong gradient
         if reduction == "none":
-            loss = torch.empty(teacher.lead, dtype=torch.float32, device=z.device)
+            loss = z.new_empty(teacher.lead, dtype=torch.float32)
             if z.shape[0]:
                 teacher.call(z, rows=loss)
         else:
-            loss = torch.empty((), dtype=torch.float32, device=z.device)
+            loss = z.new_empty((), dtype=torch.float32)
             teacher.call(z, total=loss, scale=scale)
         return loss
 
@@ -162,7 +173,7 @@ class _DistillLoss(torch.autograd.Function):
     def gradient(ctx, gout):
         logits = ctx.saved_tensors[0]
         z = _rows(logits, "logits")
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        grad = z.new_empty(logits.shape)
         if z.shape[0]:
             if gout.dtype != torch.float32 or not gout.is_contiguous():
                 gout = gout.float().contiguous()
@@ -202,15 +213,15 @@ def distill_loss_grad(logits: torch.Tensor, top_values: torch.Tensor, top_idx: t
     """(loss, d loss / d logits) of `distill_loss` in one pass over the logits: for training loops that hand the gradient on themselves
     (`logits.backward(grad)`), with the loss's own cotangent 1.  With reduction 'none' the gradient is that of the rows' sum."""
     t = _Teacher(logits, top_values, top_idx, tail, temperature, weight)
-    z = _rows(logits.detach(), "logits")
+    z = _rows(logits, "logits")
     scale = _scale(reduction, z.shape[0])
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    grad = z.new_empty(logits.shape)
     if reduction == "none":
-        loss = torch.empty(t.lead, dtype=torch.float32, device=z.device)
+        loss = z.new_empty(t.lead, dtype=torch.float32)
         if z.shape[0]:
             t.call(z, rows=loss, grad=grad)
     else:
-        loss = torch.empty((), dtype=torch.float32, device=z.device)
+        loss = z.new_empty((), dtype=torch.float32)
         t.call(z, total=loss, grad=grad, scale=scale)
     return loss, grad
 
@@ -233,9 +244,10 @@ def verify_draft(target_probs: torch.Tensor, draft_tokens: torch.Tensor, uniform
     u q(x) < p(x) (exact, in 64 bits); the draw is from max(p - q, 0) at the refused draft, from the target's next row if none was refused,
     from the target's own row where nothing is left of it over the draft, and -1 where that row is empty.  A token outside [0, V) is refused."""
     ty = _type(target_probs, "target_probs")
-    _need_cuda(draft_tokens, "draft_tokens")
-    _need_cuda(uniforms, "uniforms")
-    if draft_tokens.dtype not in (torch.int32, torch.int64):
+    dev = target_probs.get_device()
+    _beside(draft_tokens, dev, "draft_tokens")
+    _beside(uniforms, dev, "uniforms")
+    if draft_tokens.dtype is not torch.int32 and draft_tokens.dtype is not torch.int64:
         raise ValueError(f"draft_tokens must be int32 or int64, got {draft_tokens.dtype}")
     if uniforms.dtype != torch.float32:
         raise ValueError(f"uniforms must be float32, got {uniforms.dtype}")
@@ -248,26 +260,26 @@ def verify_draft(target_probs: torch.Tensor, draft_tokens: torch.Tensor, uniform
     if target_probs.shape != (*lead, G + 1, V) or uniforms.shape != (*lead, G + 1):
         raise ValueError(f"target_probs must be {(*lead, G + 1, V)} and uniforms {(*lead, G + 1)}, got {tuple(target_probs.shape)} "
                          f"and {tuple(uniforms.shape)}")
-    p = _steps(target_probs.detach())
+    p = _steps(target_probs)
     q = None
     if draft_probs is not None and G > 0:
         if draft_probs.shape != (*lead, G, V) or draft_probs.dtype != target_probs.dtype:
             raise ValueError(f"draft_probs must be {(*lead, G, V)} of {target_probs.dtype}, got {tuple(draft_probs.shape)} of {draft_probs.dtype}")
-        _need_cuda(draft_probs, "draft_probs")
-        q = _steps(draft_probs.detach())
+        _beside(draft_probs, dev, "draft_probs")
+        q = _steps(draft_probs)
     B = p.shape[0]
     x, u = draft_tokens.contiguous(), uniforms.contiguous()
     if lengths is not None:
-        _need_cuda(lengths, "lengths")
+        _beside(lengths, dev, "lengths")
         if lengths.shape != lead or lengths.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"lengths must be {tuple(lead)} int32 or int64, got {tuple(lengths.shape)} {lengths.dtype}")
         lengths = lengths.to(torch.int32).contiguous()
-    tokens = torch.empty(*lead, G + 1, dtype=torch.int32, device=p.device)
-    accepted = torch.empty(lead, dtype=torch.int32, device=p.device)
+    tokens = p.new_empty((*lead, G + 1), dtype=torch.int32)
+    accepted = p.new_empty(lead, dtype=torch.int32)
     lib, ws, n = L.lib(), None, 0
     if V > 1024:
         n = lib.elg_verify_ws_bytes(B, V, ty)
-        ws = torch.empty(n, dtype=torch.uint8, device=p.device) if n else None
+        ws = p.new_empty(n, dtype=torch.uint8) if n else None
     L.check(lib.elg_verify_draft(_p(p), p.stride(0), p.stride(1), _p(q), q.stride(0) if q is not None else 0,
                                      q.stride(1) if q is not None else 0, ty, _p(x), int(x.dtype == torch.int64), G, _p(u), G + 1,
                                      _p(lengths), B, G, V, _p(tokens), _p(accepted), _p(ws), n, _stream()), "elg_verify_draft")
