@@ -417,183 +417,220 @@ __global__ __launch_bounds__(SEG_T) void distill_join_kernel(const DistillArgs A
     if (first && s.live && (whole ? c_of >= c_lo && c_of < c_end : seg == grid_segs - 1)) entry_grad<DT>(grow, en, eidx, ee, k, only, s, A.c2, mine);
 }
 
+// ---------------------------------------------------------------------------------------------------------------------------------
 // Short rows, G lanes per row (16: four rows to a wave; 64: one).  Lane l holds the nodes n = i G + l, i < NE, and the entries
-// j = e G + l, e < KE, in registers; a row is read and written in runs of G elements, whatever its alignment.  The row's teacher masses are
-// spread over a row of LDS, one float per node, where the lane that owns the node picks them up: -0 marks a node of no entry, and
-// -0 + q = q exactly.  Waves never wait for each other.
+// j = e G + l, e < KE, in registers; a row is read and written in runs of G elements, whatever its alignment, and the next row is on its way
+// while this one is worked on (the stores of a row would otherwise stand between it and the next row's loads).
+// A row of LDS, one float per node, carries what nodes and entries have to tell each other: first the nodes' logits, picked up by the entries,
+// then the entries' teacher masses, picked up by the nodes (-0 marks a node of no entry, and -0 + q = q exactly).  Node n lies at
+// (n % G) PN + n / G there: a lane's own nodes are side by side, so that it moves them 16 bytes at a time, PN apart so that no two lanes'
+// banks meet (LDS cycles, at 8 to 10 for a 4-byte
+// access of a wave, weigh as much as the arithmetic).  Waves never wait for each other.
 template <int G> __device__ __forceinline__ float gsum(float v) { return G == 16 ? row16_sum(v) : wave_sum(v); }
 template <int G> __device__ __forceinline__ float gmax(float v) { return G == 16 ? row16_max(v) : wave_max(v); }
 
-template <int DT, int G, int NE, int KE, bool TAIL>
+template <int DT, int G, int NE, int KE>
+struct ShortRow {
+    float w, z[NE], t[KE];
+    int i[KE];
+    __device__ __forceinline__ void load(const DistillArgs& A, long long r, float weight, int l, bool plain_entries) {
+        w = weight;
+#pragma unroll
+        for (int e = 0; e < KE; ++e) { i[e] = -1; t[e] = ELG_NEG_INF; }
+#pragma unroll
+        for (int n = 0; n < NE; ++n) z[n] = ELG_NEG_INF;
+        if (w == 0.f) return;             // (a NaN weight is not 0)
+        const int k = A.k, V = A.V;
+        if (plain_entries) {
+            const int* ti = reinterpret_cast<const int*>(A.ti) + r * k + l;
+            const float* tv = reinterpret_cast<const float*>(A.tv) + r * k + l;
+#pragma unroll
+            for (int e = 0; e < KE; ++e)
+                if (l < k - e * G) {
+                    i[e] = ti[e * G];
+                    t[e] = tv[e * G];
+                }
+        } else {
+#pragma unroll
+            for (int e = 0; e < KE; ++e)
+                if (l < k - e * G) {
+                    const long long n = index_any(A.ti, r * k + e * G + l, A.ti_wide);
+                    i[e] = n >= 0 && n < V ? (int)n : -1;
+                    t[e] = elem_any(A.tv, r * k + e * G + l, A.tv_type);
+                }
+        }
+        const elem_t<DT>* row = reinterpret_cast<const elem_t<DT>*>(A.z + r * A.z_stride) + l;
+#pragma unroll
+        for (int n = 0; n < NE; ++n) {
+            if (n * G + G <= V) z[n] = (float)row[n * G];
+            else if (l < V - n * G) z[n] = (float)row[n * G];
+        }
+    }
+};
+
+template <int DT, int G, int NE, int KE>
 __global__ __launch_bounds__(256) void distill_small_kernel(const DistillArgs A) {
-    // a row of LDS is padded so that the rows of a wave's four groups start 16 banks apart
-    constexpr int RW = 64 / G, P = G * NE + (G == 16 ? 16 : 0);
-    __shared__ float qs_all[4 * RW * P];
+    constexpr int RW = 64 / G, PN = NE == 4 ? 4 : NE + 4, P = G * PN + 4;
+    constexpr bool AHEAD = NE <= 16;      // registers for the next row too
+    __shared__ __attribute__((aligned(16))) float qs_all[4 * RW * P];
     __shared__ double dred[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane / G, l = lane % G, V = A.V, k = A.k;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane / G, l0 = lane % G, V = A.V;
     float* qs = qs_all + (wave * RW + g) * P;
     const bool plain_entries = A.tv_type == ELG_F32 && !A.ti_wide;
     const float inv_tau = 1.f / A.tau;
+    const long long step = (long long)gridDim.x * 4 * RW;
+    auto weight_of = [&](long long r) { return r < A.R ? A.weight ? A.weight[r] : 1.f : 0.f; };
     double lacc = 0.0;
-    for (long long r0 = ((long long)blockIdx.x * 4 + wave) * RW; r0 < A.R; r0 += (long long)gridDim.x * 4 * RW) {
+    long long r0 = ((long long)blockIdx.x * 4 + wave) * RW;
+    float w_next = weight_of(r0 + step + g);          // weights are two rows ahead: they decide whether the next row is loaded
+    ShortRow<DT, G, NE, KE> next;
+    next.load(A, r0 + g, weight_of(r0 + g), l0, plain_entries);
+    for (; r0 < A.R; r0 += step) {
         const long long r = r0 + g;
         const bool valid = r < A.R;
-        const float w = !valid ? 0.f : A.weight ? A.weight[r] : 1.f;
-        const bool on = w != 0.f;
-        const elem_t<DT>* row = reinterpret_cast<const elem_t<DT>*>(A.z + (valid ? r : 0) * A.z_stride);
-        // ---- entries and nodes
-        const int kk = on ? k : 0, vv = on ? V : 0;
-        int ei[KE];
-        float et[KE], zi[KE];
-        if (plain_entries) {
-            const int* ti = reinterpret_cast<const int*>(A.ti) + r * k;
-            const float* tv = reinterpret_cast<const float*>(A.tv) + r * k;
+        int l = l0;
+        asm volatile("" : "+v"(l));       // the comparisons with node numbers are formed where they are used, not kept across the rows
+        ShortRow<DT, G, NE, KE> x = next;
+        // ---- the entries' logits
+        float* mine = qs + l * PN;
+        wave_lds_fence();
 #pragma unroll
-            for (int e = 0; e < KE; ++e) {
-                const int j = e * G + l;
-                ei[e] = j < kk ? ti[j] : -1;
-                et[e] = j < kk ? tv[j] : ELG_NEG_INF;
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < KE; ++e) {
-                const int j = e * G + l;
-                ei[e] = -1;
-                et[e] = ELG_NEG_INF;
-                if (j < kk) {
-                    const long long i = index_any(A.ti, r * k + j, A.ti_wide);
-                    ei[e] = i >= 0 && i < V ? (int)i : -1;
-                    et[e] = elem_any(A.tv, r * k + j, A.tv_type);
-                }
-            }
-        }
-        float v[NE];
-#pragma unroll
-        for (int i = 0; i < NE; ++i) v[i] = i * G + l < vv ? (float)row[i * G + l] : ELG_NEG_INF;
+        for (int n = 0; n < NE; n += 4) *reinterpret_cast<float4*>(mine + n) = make_float4(x.z[n], x.z[n + 1], x.z[n + 2], x.z[n + 3]);
+        wave_lds_fence();
+        float zi[KE];
+        int at[KE];                       // an entry's place in LDS, -1: absent
 #pragma unroll
         for (int e = 0; e < KE; ++e) {
-            const bool ok = (unsigned)ei[e] < (unsigned)V;
-            ei[e] = ok ? ei[e] : -1;
-            et[e] = ok ? et[e] : ELG_NEG_INF;
-            zi[e] = ok ? (float)row[ei[e]] : ELG_NEG_INF;
+            const bool ok = (unsigned)x.i[e] < (unsigned)V;
+            at[e] = ok ? (x.i[e] % G) * PN + x.i[e] / G : -1;
+            x.t[e] = ok ? x.t[e] : ELG_NEG_INF;
+            zi[e] = ok ? qs[at[e]] : ELG_NEG_INF;
         }
-        float a = TAIL && on ? A.tail[r] : 0.f;
+        float a = A.tail && valid ? A.tail[r] : 0.f;
+        const float w_after = weight_of(r + 2 * step);
+        if (AHEAD) next.load(A, r + step, w_next, l, plain_entries);
         a = a > 1.f ? 1.f : a < 0.f ? 0.f : a;
-        // ---- the teacher's masses
-        float tm = et[0];
+        // ---- the teacher's masses, still to be scaled
+        float tm = x.t[0], mz = zi[0];
 #pragma unroll
-        for (int e = 1; e < KE; ++e) tm = fmaxf(tm, et[e]);
+        for (int e = 1; e < KE; ++e) {
+            tm = fmaxf(tm, x.t[e]);
+            mz = fmaxf(mz, zi[e]);
+        }
         tm = gmax<G>(tm);
+        mz = gmax<G>(mz);
         tm = tm > ELG_NEG_INF ? tm : 0.f;
-        float q[KE], st = 0.f;
+        const float z_ref = mz > ELG_NEG_INF ? mz : 0.f;
+        float q[KE], st = 0.f, sz = 0.f;
 #pragma unroll
         for (int e = 0; e < KE; ++e) {
-            q[e] = ei[e] >= 0 ? ex2((et[e] - tm) * A.c2) : 0.f;
+            q[e] = at[e] >= 0 ? ex2((x.t[e] - tm) * A.c2) : 0.f;
             st += q[e];
         }
-        st = gsum<G>(st);
-        const float qscale = st <= 0.f ? 0.f : (1.f - a) * __builtin_amdgcn_rcpf(st);
-#pragma unroll
-        for (int e = 0; e < KE; ++e) q[e] *= qscale;
         auto clear = [&]() {
             wave_lds_fence();
 #pragma unroll
-            for (int i = 0; i < NE; ++i) qs[i * G + l] = -0.f;
+            for (int n = 0; n < NE; n += 4) *reinterpret_cast<float4*>(mine + n) = make_float4(-0.f, -0.f, -0.f, -0.f);
             wave_lds_fence();
         };
+        constexpr int MARK = (int)0x80000000;
         clear();
-        bool twice = false;
+        // Is some node listed twice?  Every entry leaves its number at its node and looks whether it is still there: two plain accesses for what
+        // a returning LDS addition of floats would tell at several times the cycles.
+        bool first[KE], twice = false;    // the first entry of its node counts it in the softmax
+#pragma unroll
+        for (int e = 0; e < KE; ++e) {
+            first[e] = at[e] >= 0;
+            if (at[e] >= 0) qs[at[e]] = i2f(e * G + l);
+        }
+        wave_lds_fence();
 #pragma unroll
         for (int e = 0; e < KE; ++e)
-            if (ei[e] >= 0) {
-                const float old = __hip_atomic_fetch_add(qs + ei[e], q[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                twice = twice || f2i(old) != (int)0x80000000;
-            }
-        if (__any(twice)) {               // some node is listed twice: add its masses again, in entry order, so that the bits are the same in every run
+            if (at[e] >= 0) twice = twice || f2i(qs[at[e]]) != e * G + l;
+        wave_lds_fence();
+#pragma unroll
+        for (int e = 0; e < KE; ++e)
+            if (at[e] >= 0) qs[at[e]] = q[e];
+        if (__any(twice)) {               // then the masses are added up in entry order
             clear();
 #pragma unroll
             for (int e = 0; e < KE; ++e)
 #pragma unroll 1
                 for (int j = 0; j < G; ++j) {
-                    if (j == l && ei[e] >= 0) qs[ei[e]] += q[e];
+                    if (j == l && at[e] >= 0) {
+                        const float old = qs[at[e]];
+                        first[e] = f2i(old) == MARK;
+                        qs[at[e]] = old + q[e];
+                    }
                     wave_lds_fence();
                 }
         }
         wave_lds_fence();
         float qv[NE];
 #pragma unroll
-        for (int i = 0; i < NE; ++i) qv[i] = qs[i * G + l];
-        // ---- the student's softmax; v becomes e^(z - its part's maximum)
-        float m, S, f_top = 1.f, f_rest = 0.f, s_rest = 0.f, m_rest = 0.f;
-        if (TAIL) {
-            float mt = ELG_NEG_INF, mr = ELG_NEG_INF;
-#pragma unroll
-            for (int i = 0; i < NE; ++i) {
-                const bool top = f2i(qv[i]) >= 0;
-                mt = fmaxf(mt, top ? v[i] : ELG_NEG_INF);
-                mr = fmaxf(mr, top ? ELG_NEG_INF : v[i]);
-            }
-            mt = gmax<G>(mt);
-            mr = gmax<G>(mr);
-            m = fmaxf(mt, mr);
-            const float m_top = mt > ELG_NEG_INF ? mt : 0.f;
-            m_rest = mr > ELG_NEG_INF ? mr : 0.f;
-            float s_top = 0.f;
-#pragma unroll
-            for (int i = 0; i < NE; ++i) {
-                const bool top = f2i(qv[i]) >= 0;
-                v[i] = ex2((v[i] - (top ? m_top : m_rest)) * A.c2);
-                s_top += top ? v[i] : 0.f;
-                s_rest += top ? 0.f : v[i];
-            }
-            s_top = gsum<G>(s_top);
-            s_rest = gsum<G>(s_rest);
-            f_top = mt > ELG_NEG_INF ? ex2((m_top - m) * A.c2) : 0.f;
-            f_rest = mr > ELG_NEG_INF ? ex2((m_rest - m) * A.c2) : 0.f;
-            S = s_top * f_top + s_rest * f_rest;
-        } else {
-            m = v[0];
-#pragma unroll
-            for (int i = 1; i < NE; ++i) m = fmaxf(m, v[i]);
-            m = gmax<G>(m);
-            const float ref = m > ELG_NEG_INF ? m : 0.f;
-            S = 0.f;
-#pragma unroll
-            for (int i = 0; i < NE; ++i) {
-                v[i] = ex2((v[i] - ref) * A.c2);
-                S += v[i];
-            }
-            S = gsum<G>(S);
+        for (int n = 0; n < NE; n += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(mine + n);
+            qv[n] = f.x; qv[n + 1] = f.y; qv[n + 2] = f.z; qv[n + 3] = f.w;
         }
-        const bool live = on && !(S <= 0.f) && !(st <= 0.f);
-        const float inv_S = __builtin_amdgcn_rcpf(S);
-        // ---- loss
-        if (A.loss_rows || A.part || A.total) {
-            float L = 0.f;
 #pragma unroll
-            for (int e = 0; e < KE; ++e) L += q[e] > 0.f || q[e] != q[e] ? q[e] * ((et[e] - tm) - (zi[e] - m)) : 0.f;
-            L = gsum<G>(L) * inv_tau;
-            if (a < 1.f) L += (1.f - a) * ln(qscale * S);
-            if (TAIL && a > TINY_MASS) L += a * (ln(a * S * __builtin_amdgcn_rcpf(s_rest)) - (m_rest - m) * inv_tau);
-            L = live ? L * (A.tau * A.tau * w) : 0.f;
+        for (int e = 0; e < KE; ++e) sz += first[e] ? ex2((zi[e] - z_ref) * A.c2) : 0.f;
+        // ---- the nodes: z becomes e^(z - the maximum of its part)
+        float mr = ELG_NEG_INF;
+#pragma unroll
+        for (int n = 0; n < NE; ++n) mr = fmaxf(mr, f2i(qv[n]) < 0 ? x.z[n] : ELG_NEG_INF);
+        mr = gmax<G>(mr);
+        const float m_rest = mr > ELG_NEG_INF ? mr : 0.f, m = fmaxf(mz, mr);
+        float sr = 0.f, sd = 0.f;
+#pragma unroll
+        for (int n = 0; n < NE; ++n) {
+            const bool rest = f2i(qv[n]) < 0;
+            x.z[n] = ex2((x.z[n] - (rest ? m_rest : z_ref)) * A.c2);
+            sr += rest ? x.z[n] : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < KE; ++e) sd += q[e] > 0.f || q[e] != q[e] ? q[e] * ((x.t[e] - tm) - (zi[e] - m)) : 0.f;
+        st = gsum<G>(st);
+        sz = gsum<G>(sz);
+        sr = gsum<G>(sr);
+        // ---- the row's scalars
+        const float f_top = mz > ELG_NEG_INF ? ex2((mz - m) * A.c2) : 0.f, f_rest = mr > ELG_NEG_INF ? ex2((mr - m) * A.c2) : 0.f;
+        const float S = sz * f_top + sr * f_rest, inv_S = __builtin_amdgcn_rcpf(S), inv_sr = __builtin_amdgcn_rcpf(sr);
+        const float q_scale = st <= 0.f ? 0.f : (1.f - a) * __builtin_amdgcn_rcpf(st);
+        const bool live = x.w != 0.f && !(S <= 0.f) && !(st <= 0.f);
+        if (A.loss_rows || A.part || A.total) {
+            float L = gsum<G>(sd) * q_scale * inv_tau;
+            if (a < 1.f) L += (1.f - a) * ln(q_scale * S);
+            if (a > TINY_MASS) L += a * (ln(a * S * inv_sr) - (m_rest - m) * inv_tau);
+            L = live ? L * (A.tau * A.tau * x.w) : 0.f;
             if (l == 0 && valid) {
                 if (A.loss_rows) A.loss_rows[r] = L * A.scale;
                 lacc += (double)L;
             }
         }
         // ---- gradient
-        if (A.grad && valid) {
-            const float cot = A.cot ? A.cot[r * A.cot_stride] : 1.f;
-            const float Gr = live ? A.scale * cot * w * A.tau : 0.f, c_top = live ? Gr * f_top * inv_S : 0.f;
-            float c_rest = c_top;
-            if (TAIL) c_rest = live ? Gr * (f_rest * inv_S - (a > 0.f && s_rest > 0.f ? a * __builtin_amdgcn_rcpf(s_rest) : 0.f)) : 0.f;
-            elem_t<DT>* grow = reinterpret_cast<elem_t<DT>*>(A.grad + r * A.g_stride);
+        if (A.grad) {
+            const float cot = A.cot && valid ? A.cot[r * A.cot_stride] : 1.f;
+            const float Gr = live ? A.scale * cot * x.w * A.tau : 0.f;
+            const float c_rest = live ? Gr * (f_rest * inv_S - (a > 0.f && sr > 0.f ? a * inv_sr : 0.f)) : 0.f;
+            const float Gq = Gr * q_scale, c_top = live ? Gr * f_top * inv_S : 0.f;
+            if (__any(!live))             // (whatever the nodes of a row without a gradient came to)
 #pragma unroll
-            for (int i = 0; i < NE; ++i) {
-                const float t = fmaf(live ? v[i] : 0.f, !TAIL || f2i(qv[i]) >= 0 ? c_top : c_rest, -Gr * qv[i]);
-                if (i * G + l < V) grow[i * G + l] = (elem_t<DT>)t;
+                for (int n = 0; n < NE; ++n) {
+                    x.z[n] = live ? x.z[n] : 0.f;
+                    qv[n] = live ? qv[n] : 0.f;
+                }
+            if (valid) {
+                elem_t<DT>* grow = reinterpret_cast<elem_t<DT>*>(A.grad + r * A.g_stride) + l;
+#pragma unroll
+                for (int n = 0; n < NE; ++n) {
+                    const float gn = fmaf(x.z[n], f2i(qv[n]) < 0 ? c_rest : c_top, -Gq * qv[n]);
+                    if (n * G + G <= V) grow[n * G] = (elem_t<DT>)gn;
+                    else if (l < V - n * G) grow[n * G] = (elem_t<DT>)gn;
+                }
             }
         }
+        if (!AHEAD) next.load(A, r + step, w_next, l, plain_entries);
+        w_next = w_after;
     }
     if (A.part || A.total) {
 #pragma unroll
@@ -626,12 +663,12 @@ constexpr int MAX_GRID = 2048;
 
 template <int DT, int G, int NE, int KE>
 void launch_small(const DistillArgs& A, int grid, hipStream_t s) {
-    if (A.tail) hipLaunchKernelGGL((distill_small_kernel<DT, G, NE, KE, true>), dim3((unsigned)grid), dim3(256), 0, s, A);
-    else hipLaunchKernelGGL((distill_small_kernel<DT, G, NE, KE, false>), dim3((unsigned)grid), dim3(256), 0, s, A);
+    hipLaunchKernelGGL((distill_small_kernel<DT, G, NE, KE>), dim3((unsigned)grid), dim3(256), 0, s, A);
 }
 
 // How a call is laid out, from its sizes alone (the scratch it needs follows from them too).
 struct Plan {
+    int lanes;                            // of a short row; 0: a workgroup or more
     bool split;
     int segs;
     bool one;                             // so few short rows that one workgroup forms their total: a launch and the scratch saved
@@ -640,10 +677,11 @@ struct Plan {
         const int vec = type == ELG_F32 ? 4 : 8;
         // rows that no workgroup can hold, or so few long ones that most of the chip would idle: measured, 6 rows of 100003 f32: 142 us a
         // workgroup each, 24 us split; 256 rows of 32000 bf16: 16 and 19 us
-        split = V > 2048 && (V > 1024 * 16 * vec || (R <= 64 && V > 1024 * vec));
+        lanes = V <= 256 ? 16 : V <= 2048 ? 64 : 0;
+        split = !lanes && (V > 1024 * 16 * vec || (R <= 64 && V > 1024 * vec));
         segs = split ? (int)((V + vec - 1 + SEG_T * SEG_C * vec - 1) / (SEG_T * SEG_C * vec)) : 0;     // a row may start inside its first 16 bytes
-        const long long rows_wg = V <= 256 ? 16 : V <= 2048 ? 4 : 1, want = (R + rows_wg - 1) / rows_wg;
-        one = V <= 2048 && want <= 8;
+        const long long rows_wg = lanes == 16 ? 16 : lanes == 64 ? 4 : 1, want = (R + rows_wg - 1) / rows_wg;
+        one = lanes && want <= 8;
         parts = split ? R : want < MAX_GRID ? want : MAX_GRID;
     }
     long long bytes(long long R) const { return one ? 0 : 8 * parts + 8 * R * segs; }
@@ -662,14 +700,14 @@ void launch(const DistillArgs& A, const Plan& P, float2* parts, hipStream_t s) {
     // chunks a row can span: its own and, unless every row starts on 16 bytes, what the first line holds in front of it
     const bool aligned = !((uintptr_t)A.z & 15) && !(A.z_stride & 15);
     const int nch = (V + (aligned ? 0 : VEC<DT> - 1) + VEC<DT> - 1) / VEC<DT>;
-    if (V <= 256) {
-        if (k > 48) V <= 128 ? launch_small<DT, 16, 8, 16>(A, grid, s) : launch_small<DT, 16, 16, 16>(A, grid, s);
-        else if (k > 16) V <= 64 ? launch_small<DT, 16, 4, 3>(A, grid, s) : V <= 128 ? launch_small<DT, 16, 8, 3>(A, grid, s) : launch_small<DT, 16, 16, 3>(A, grid, s);
-        else if (V <= 32) launch_small<DT, 16, 2, 1>(A, grid, s);
-        else V <= 64 ? launch_small<DT, 16, 4, 1>(A, grid, s) : V <= 128 ? launch_small<DT, 16, 8, 1>(A, grid, s) : launch_small<DT, 16, 16, 1>(A, grid, s);
-    } else if (V <= 2048) {
-        if (k <= 64) V <= 512 ? launch_small<DT, 64, 8, 1>(A, grid, s) : V <= 1024 ? launch_small<DT, 64, 16, 1>(A, grid, s) : launch_small<DT, 64, 32, 1>(A, grid, s);
-        else V <= 512 ? launch_small<DT, 64, 8, 4>(A, grid, s) : V <= 1024 ? launch_small<DT, 64, 16, 4>(A, grid, s) : launch_small<DT, 64, 32, 4>(A, grid, s);
+    auto fits = [&](int g, int ne) { return V <= g * ne; };
+    if (P.lanes == 16) {
+        if (k > 48) fits(16, 8) ? launch_small<DT, 16, 8, 16>(A, grid, s) : launch_small<DT, 16, 16, 16>(A, grid, s);
+        else if (k > 16) fits(16, 4) ? launch_small<DT, 16, 4, 3>(A, grid, s) : fits(16, 8) ? launch_small<DT, 16, 8, 3>(A, grid, s) : launch_small<DT, 16, 16, 3>(A, grid, s);
+        else fits(16, 4) ? launch_small<DT, 16, 4, 1>(A, grid, s) : fits(16, 8) ? launch_small<DT, 16, 8, 1>(A, grid, s) : launch_small<DT, 16, 16, 1>(A, grid, s);
+    } else if (P.lanes == 64) {
+        if (k <= 64) fits(64, 8) ? launch_small<DT, 64, 8, 1>(A, grid, s) : fits(64, 16) ? launch_small<DT, 64, 16, 1>(A, grid, s) : launch_small<DT, 64, 32, 1>(A, grid, s);
+        else fits(64, 8) ? launch_small<DT, 64, 8, 4>(A, grid, s) : fits(64, 16) ? launch_small<DT, 64, 16, 4>(A, grid, s) : launch_small<DT, 64, 32, 4>(A, grid, s);
     } else if (P.split) {
         const int grad_segs = A.grad ? P.segs : 1;
         hipLaunchKernelGGL((distill_part_kernel<DT>), dim3((unsigned)(A.R * P.segs)), dim3(SEG_T), 0, s, A, parts, P.segs);
