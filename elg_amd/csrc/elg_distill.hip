@@ -37,7 +37,10 @@ struct DistillArgs {
 };
 
 constexpr float TINY_MASS = 1e-36f;       // a (log a - log p_rest) below this is nothing in f32
-__device__ __forceinline__ float ln(float x) { return __builtin_amdgcn_logf(x) * 0.6931471805599453f; }
+// The loss is formed in base 2, every difference of logits times the one rounded c2 of the exponentials, and brought to base e at its end: with
+// 1 / tau rounded apart from c2 the two would differ by 2^-24 of every difference, the same way in every row.
+constexpr float LN2 = 0.6931471805599453f;
+__device__ __forceinline__ float lg2(float x) { return __builtin_amdgcn_logf(x); }       // v_log_f32
 
 // ---------------------------------------------------------------------------------------------------------------------------------
 // Long rows: T >= ELG_TOP_MAX_K threads, thread j < k holding entry j, the row in 16-byte chunks.  A bitmap in LDS tells a chunk which of its
@@ -87,11 +90,10 @@ struct RowScalars {
         live = !(S <= 0.f) && !(st <= 0.f);
         inv_S = __builtin_amdgcn_rcpf(S);
         q_scale = st <= 0.f ? 0.f : (1.f - a) * __builtin_amdgcn_rcpf(st);
-        const float inv_tau = 1.f / A.tau;
-        float L = sd * q_scale * inv_tau;
-        if (a < 1.f) L += (1.f - a) * ln(q_scale * S);
-        if (a > TINY_MASS) L += a * (ln(a * S * __builtin_amdgcn_rcpf(sr)) - (m_rest - m) * inv_tau);
-        loss = live ? L * (A.tau * A.tau * w) : 0.f;
+        float L = sd * q_scale * A.c2;
+        if (a < 1.f) L += (1.f - a) * lg2(q_scale * S);
+        if (a > TINY_MASS) L += a * (lg2(a * S * __builtin_amdgcn_rcpf(sr)) - (m_rest - m) * A.c2);
+        loss = live ? L * (LN2 * A.tau * A.tau * w) : 0.f;
         const float cot = A.cot ? A.cot[r * A.cot_stride] : 1.f;
         G = live ? A.scale * cot * w * A.tau : 0.f;
         c_rest = live ? G * (f_rest * inv_S - (a > 0.f && sr > 0.f ? a * __builtin_amdgcn_rcpf(sr) : 0.f)) : 0.f;
@@ -477,7 +479,6 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistillArgs A)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane / G, l0 = lane % G, V = A.V;
     float* qs = qs_all + (wave * RW + g) * P;
     const bool plain_entries = A.tv_type == ELG_F32 && !A.ti_wide;
-    const float inv_tau = 1.f / A.tau;
     const long long step = (long long)gridDim.x * 4 * RW;
     auto weight_of = [&](long long r) { return r < A.R ? A.weight ? A.weight[r] : 1.f : 0.f; };
     double lacc = 0.0;
@@ -598,10 +599,10 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistillArgs A)
         const float q_scale = st <= 0.f ? 0.f : (1.f - a) * __builtin_amdgcn_rcpf(st);
         const bool live = x.w != 0.f && !(S <= 0.f) && !(st <= 0.f);
         if (A.loss_rows || A.part || A.total) {
-            float L = gsum<G>(sd) * q_scale * inv_tau;
-            if (a < 1.f) L += (1.f - a) * ln(q_scale * S);
-            if (a > TINY_MASS) L += a * (ln(a * S * inv_sr) - (m_rest - m) * inv_tau);
-            L = live ? L * (A.tau * A.tau * x.w) : 0.f;
+            float L = gsum<G>(sd) * q_scale * A.c2;
+            if (a < 1.f) L += (1.f - a) * lg2(q_scale * S);
+            if (a > TINY_MASS) L += a * (lg2(a * S * inv_sr) - (m_rest - m) * A.c2);
+            L = live ? L * (LN2 * A.tau * A.tau * x.w) : 0.f;
             if (l == 0 && valid) {
                 if (A.loss_rows) A.loss_rows[r] = L * A.scale;
                 lacc += (double)L;

@@ -71,80 +71,262 @@ struct Count {                            // block-wide counts; one barrier each
     }
 };
 
-// One workgroup per row.  C > 0: the row stays in registers, C chunks a thread; C = 0: every pass reads it again.
-template <int DT, int T, int C>
-__global__ __launch_bounds__(T) void top_row_kernel(const TopArgs A) {
-    __shared__ unsigned long long cand[TOP_CAP];
-    __shared__ unsigned long long win[ELG_TOP_MAX_K];
-    __shared__ float fred[2 * 2 * (T / 64)];
-    __shared__ int cred[2 * (T / 64)];
-    __shared__ int n_cand;
-    const int tid = threadIdx.x, V = A.V, k = A.k;
-    BlockRed<T / 64> red(fred);
-    Count<T> cnt(cred);
-    for (long long r = blockIdx.x; r < A.R; r += gridDim.x) {
-        const char* row = A.z + r * A.stride_bytes;
-        const int shift = shift_of<DT>(row), nch = (shift + V + VEC<DT> - 1) / VEC<DT>;
-        u32x4 zr[C ? C : 1];
-        if (C) {
+// A register of one f32 or two 16-bit elements <-> the order keys of the same width, in place: three operations for either.  These keys
+// tell -0 from 0 and put NaN at both ends; the callers see to both.
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+template <int DT> struct WordKey {                                    // two 16-bit keys
+    static constexpr unsigned NEG_INF = DT == ELG_BF16 ? 0x007Fu : 0x03FFu, POS_INF = DT == ELG_BF16 ? 0xFF80u : 0xFC00u, ZERO = 0x8000u, TOP = 0xFFFFu;
+    static __device__ __forceinline__ unsigned to(unsigned w) {
+        const s16x2 sign = __builtin_bit_cast(s16x2, w) >> 15;
+        return w ^ (__builtin_bit_cast(unsigned, sign) | 0x80008000u);
+    }
+    static __device__ __forceinline__ unsigned from(unsigned k) {
+        const s16x2 sign = __builtin_bit_cast(s16x2, k) >> 15;
+        return k ^ (~__builtin_bit_cast(unsigned, sign) | 0x80008000u);
+    }
+    static __device__ __forceinline__ unsigned hi(unsigned a, unsigned b) {
+        return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+    }
+    static __device__ __forceinline__ unsigned lo(unsigned a, unsigned b) {
+        return __builtin_bit_cast(unsigned, __builtin_elementwise_min(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+    }
+    static __device__ __forceinline__ unsigned highest(unsigned w) { return max(w >> 16, w & 0xFFFFu); }
+    static __device__ __forceinline__ unsigned lowest(unsigned w) { return min(w >> 16, w & 0xFFFFu); }
+    static __device__ __forceinline__ unsigned at(const u32x4& z, int e) { return (e & 1) ? z[e >> 1] >> 16 : z[e >> 1] & 0xFFFFu; }
+};
+template <> struct WordKey<ELG_F32> {
+    static constexpr unsigned NEG_INF = KEY_NEG_INF, POS_INF = 0xFF800000u, ZERO = 0x80000000u, TOP = 0xFFFFFFFFu;
+    static __device__ __forceinline__ unsigned to(unsigned w) { return w ^ ((unsigned)((int)w >> 31) | 0x80000000u); }
+    static __device__ __forceinline__ unsigned from(unsigned k) { return k ^ (~(unsigned)((int)k >> 31) | 0x80000000u); }
+    static __device__ __forceinline__ unsigned hi(unsigned a, unsigned b) { return max(a, b); }
+    static __device__ __forceinline__ unsigned lo(unsigned a, unsigned b) { return min(a, b); }
+    static __device__ __forceinline__ unsigned highest(unsigned w) { return w; }
+    static __device__ __forceinline__ unsigned lowest(unsigned w) { return w; }
+    static __device__ __forceinline__ unsigned at(const u32x4& z, int e) { return z[e]; }
+};
+// the key of one element given as a float
+template <int DT>
+__device__ __forceinline__ unsigned word_key(float f) {
+    if constexpr (DT == ELG_F32) return WordKey<DT>::to((unsigned)f2i(f));
+    else if constexpr (DT == ELG_BF16) return WordKey<DT>::to((unsigned)f2i(f) >> 16) & 0xFFFFu;
+    else return WordKey<DT>::to((unsigned)__builtin_bit_cast(unsigned short, (_Float16)f)) & 0xFFFFu;
+}
+
+template <int T>
+struct TopShared {
+    unsigned long long cand[TOP_CAP];
+    unsigned long long win[ELG_TOP_MAX_K];
+    float fred[2 * 2 * (T / 64)];
+    int cred[2 * (T / 64)];
+    unsigned kred[2 * (T / 64)];
+    int n_cand;
+};
+
+// `need` elements of order key `key`, lowest indices first, into win[at ...]: the row is read from its start as far as that takes
+template <int DT, int T>
+__device__ __forceinline__ void take_ties(const void* row, int V, unsigned key, int at, int need, unsigned long long* win, Count<T>& cnt) {
+    const int tid = threadIdx.x, shift = shift_of<DT>(row), nch = (shift + V + VEC<DT> - 1) / VEC<DT>;
+    for (int c0 = 0; need > 0 && c0 < nch; c0 += T) {
+        const int c = c0 + tid;
+        unsigned hit = 0;
+        if (c < nch) {
+            float v[VEC<DT>];
+            unpack<DT>(load_chunk<DT>(row, shift, V, c, 0u), v);
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                constexpr unsigned pad = PAD_NEG_INF<DT>;
-                zr[c] = tid + c * T < nch ? load_chunk<DT>(row, shift, V, tid + c * T, pad) : u32x4{pad, pad, pad, pad};
+            for (int e = 0; e < VEC<DT>; ++e) {
+                const int n = c * VEC<DT> + e - shift;
+                if (n >= 0 && n < V && order_key(v[e]) == key) hit |= 1u << e;
             }
         }
-        // f(key, index) for every element of this thread; positions outside the row come as closed nodes
-        auto each = [&](auto&& f) {
-            if (C) {
-                int n0 = tid * VEC<DT> - shift;
-                asm volatile("" : "+v"(n0));          // node numbers are formed where they are used, not kept in registers for the next pass
-#pragma unroll
-                for (int c = 0; c < C; ++c) {
-                    float v[VEC<DT>];
-                    asm volatile("" : "+v"(zr[c]));   // and so are the keys
-                    unpack<DT>(zr[c], v);
-#pragma unroll
-                    for (int e = 0; e < VEC<DT>; ++e) f(order_key(v[e]), n0 + c * T * VEC<DT> + e);
-                }
+        int before;
+        const int tot = cnt.scan(__popc(hit), before);
+        for (; hit && before < need; ++before) {
+            const int e = __ffs(hit) - 1;
+            hit &= hit - 1;
+            win[at + before] = composite(key, c * VEC<DT> + e - shift);
+        }
+        at += min(tot, need);
+        need -= min(tot, need);
+    }
+}
+
+// the candidates in order into win (the first k of them); what the others of them and the rest weigh
+template <int DT, int T>
+__device__ __forceinline__ void finish_row(const TopArgs& A, long long r, const void* row, int found, unsigned tie_key, int tie_need, float rest, bool rest_known,
+                                           TopShared<T>& sh, Count<T>& cnt, BlockRed<T / 64>& red) {
+    const int tid = threadIdx.x, k = A.k;
+    // rank by counting; composites are unique
+    for (int i = tid; i < found; i += T) {
+        const unsigned long long me = sh.cand[i];
+        int rank = 0;
+        for (int j = 0; j < found; ++j) rank += sh.cand[j] > me;
+        if (rank < k) sh.win[rank] = me;
+    }
+    take_ties<DT, T>(row, A.V, tie_key, min(found, k), tie_need, sh.win, cnt);
+    __syncthreads();
+    for (int i = tid; i < k; i += T) {
+        const unsigned long long w = sh.win[i];
+        reinterpret_cast<elem_t<DT>*>(A.values)[r * k + i] = (elem_t<DT>)key_value((unsigned)(w >> 32));
+        A.idx[r * k + i] = (int)~(unsigned)w;
+    }
+    if (A.tail) {
+        // mass outside the winners: summed apart from the winners' own, so that a small tail keeps its digits
+        const unsigned long long last = sh.win[k - 1];
+        const float m = key_value((unsigned)(sh.win[0] >> 32));
+        float top = 0.f;
+        if (!(m > ELG_NEG_INF || m != m)) rest = 0.f;           // no open node: nothing to weigh
+        else {
+            for (int i = tid; i < k; i += T) top += ex2((key_value((unsigned)(sh.win[i] >> 32)) - m) * A.c2);
+            if (rest_known) {
+                for (int i = tid; i < found; i += T)
+                    if (sh.cand[i] < last) rest += ex2((key_value((unsigned)(sh.cand[i] >> 32)) - m) * A.c2);
             } else {
+                const int shift = shift_of<DT>(row), nch = (shift + A.V + VEC<DT> - 1) / VEC<DT>;
+                rest = 0.f;
                 for (int c = tid; c < nch; c += T) {
                     float v[VEC<DT>];
-                    unpack<DT>(load_chunk<DT>(row, shift, V, c, PAD_NEG_INF<DT>), v);
+                    unpack<DT>(load_chunk<DT>(row, shift, A.V, c, PAD_NEG_INF<DT>), v);
 #pragma unroll
-                    for (int e = 0; e < VEC<DT>; ++e) f(order_key(v[e]), c * VEC<DT> + e - shift);
+                    for (int e = 0; e < VEC<DT>; ++e)
+                        if (composite(order_key(v[e]), c * VEC<DT> + e - shift) < last) rest += ex2((v[e] - m) * A.c2);
                 }
             }
-        };
-        // r elements equal to `key`, lowest indices first, into win[at ...]; the last one's index is the same for every thread
-        auto ties = [&](unsigned key, int at, int need) {
-            for (int c0 = 0; need > 0 && c0 < nch; c0 += T) {
-                const int c = c0 + tid;
-                unsigned hit = 0;
-                if (c < nch) {
-                    float v[VEC<DT>];
-                    unpack<DT>(load_chunk<DT>(row, shift, V, c, 0u), v);
+        }
+        const float2 s = red.sum2(top, rest);
+        if (tid == 0) A.tail[r] = s.x + s.y > 0.f || s.x != s.x || s.y != s.y ? s.y / (s.x + s.y) : 0.f;
+    }
+    __syncthreads();                      // win, cand and n_cand are written again by the next row
+}
+
+// A row by order keys of whole elements, read again by every pass: rows no workgroup can hold, rows with NaN, rows with so many equal values
+// that the bound does not separate them.
+template <int DT, int T>
+__device__ __noinline__ void top_row_again(const TopArgs& A, long long r, TopShared<T>& sh) {
+    __syncthreads();                      // the reductions' buffers start over
+    BlockRed<T / 64> red(sh.fred);
+    Count<T> cnt(sh.cred);
+    const char* row = A.z + r * A.stride_bytes;
+    const int tid = threadIdx.x, V = A.V, k = A.k, shift = shift_of<DT>(row), nch = (shift + V + VEC<DT> - 1) / VEC<DT>;
+    // f(key, index) for every element of this thread; positions outside the row come as closed nodes
+    auto each = [&](auto&& f) {
+        for (int c = tid; c < nch; c += T) {
+            float v[VEC<DT>];
+            unpack<DT>(load_chunk<DT>(row, shift, V, c, PAD_NEG_INF<DT>), v);
 #pragma unroll
-                    for (int e = 0; e < VEC<DT>; ++e) {
-                        const int n = c * VEC<DT> + e - shift;
-                        if (n >= 0 && n < V && order_key(v[e]) == key) hit |= 1u << e;
-                    }
-                }
-                int before;
-                const int tot = cnt.scan(__popc(hit), before);
-                for (; hit && before < need; ++before) {
-                    const int e = __ffs(hit) - 1;
-                    hit &= hit - 1;
-                    win[at + before] = composite(key, c * VEC<DT> + e - shift);
-                }
-                at += min(tot, need);
-                need -= min(tot, need);
+            for (int e = 0; e < VEC<DT>; ++e) f(order_key(v[e]), c * VEC<DT> + e - shift);
+        }
+    };
+    // ---- the threads' maxima over open nodes, and a bound from them
+    unsigned kmax = 0;
+    each([&](unsigned key, int) { if (key > KEY_NEG_INF) kmax = max(kmax, key); });
+    if (tid == 0) sh.n_cand = 0;
+    unsigned lo = KEY_NEG_INF + 1, hi = 0xFFFFFFFFu;
+    if (cnt.of(kmax >= lo) >= k) {
+        while (lo < hi) {
+            const unsigned mid = lo + (hi - lo) / 2 + 1;
+            const int c = cnt.of(kmax >= mid);
+            if (c >= k) {
+                lo = mid;
+                if (c == k) break;
+            } else hi = mid - 1;
+        }
+    }
+    if (kmax >= lo)
+        each([&](unsigned key, int n) {
+            if (key >= lo) {
+                const int p = atomicAdd(&sh.n_cand, 1);
+                if (p < TOP_CAP) sh.cand[p] = composite(key, n);
             }
-        };
-        // ---- the threads' maxima over open nodes, and the largest of all
-        unsigned kmax = 0;
-        each([&](unsigned key, int) { if (key > KEY_NEG_INF) kmax = max(kmax, key); });
-        if (tid == 0) n_cand = 0;
-        unsigned lo = KEY_NEG_INF + 1, hi = 0xFFFFFFFFu;
+        });
+    __syncthreads();
+    int found = sh.n_cand, tie_need = 0;
+    unsigned tie_key = 0;
+    if (found > TOP_CAP) {
+        // the k-th largest key of all elements: count(>= lo) >= k holds throughout
+        hi = 0xFFFFFFFFu;
+        while (lo < hi) {
+            const unsigned mid = lo + (hi - lo) / 2 + 1;
+            int c = 0;
+            each([&](unsigned key, int) { c += key >= mid; });
+            int before;
+            c = cnt.scan(c, before);
+            if (c >= k) {
+                lo = mid;
+                if (c == k) break;
+            } else hi = mid - 1;
+        }
+        if (tid == 0) sh.n_cand = 0;
+        __syncthreads();
+        each([&](unsigned key, int n) {
+            if (key > lo) sh.cand[atomicAdd(&sh.n_cand, 1)] = composite(key, n);       // at most k of them
+        });
+        __syncthreads();
+        found = sh.n_cand;
+        tie_key = lo;
+        tie_need = k - found;
+    } else if (found < k) {
+        tie_key = KEY_NEG_INF;                                                   // closed nodes fill the rest
+        tie_need = k - found;
+    }
+    finish_row<DT, T>(A, r, row, found, tie_key, tie_need, 0.f, false, sh, cnt, red);
+}
+
+// One workgroup per row, the row in registers as order keys, C chunks a thread.  One pass for the threads' maxima, one that gathers the
+// candidates and sums the exponentials of everything below the bound.
+template <int DT, int T, int C>
+__global__ __launch_bounds__(T, 4) void top_row_kernel(const TopArgs A) {
+    using W = WordKey<DT>;
+    __shared__ TopShared<T> sh;
+    const int tid = threadIdx.x, k = A.k;
+    BlockRed<T / 64> red(sh.fred);
+    Count<T> cnt(sh.cred);
+    for (long long r = blockIdx.x; r < A.R; r += gridDim.x) {
+        const char* row = A.z + r * A.stride_bytes;
+        const Span<DT> sp(row, A.V);
+        auto place = [&]() { int t = tid; asm volatile("" : "+v"(t)); return t; };      // (see distill_row_kernel)
+        u32x4 z[C];
+        const int t0 = place();
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            constexpr unsigned pad = PAD_NEG_INF<DT>;
+            z[c] = u32x4{pad, pad, pad, pad};
+            if (t0 >= sp.c_lo - c * T && t0 < sp.c_hi - c * T) z[c] = sp.chunk(t0 + c * T);
+        }
+        const int edge = sp.edge(tid);
+        const float ze = edge >= 0 ? elem<DT>(row, edge) : ELG_NEG_INF;
+        // ---- keys, the threads' extremes
+        unsigned mx = 0u, mn = 0xFFFFFFFFu;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const unsigned w = W::to(z[c][i]);
+                z[c][i] = w;
+                mx = W::hi(mx, w);
+                mn = W::lo(mn, w);
+            }
+            asm volatile("" : "+v"(z[c]), "+v"(mx), "+v"(mn));
+        }
+        unsigned kmax = W::highest(mx), kmin = W::lowest(mn);
+        if (edge >= 0) {
+            kmax = max(kmax, word_key<DT>(ze));
+            kmin = min(kmin, word_key<DT>(ze));
+        }
+        unsigned best = kmax;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) best = max(best, (unsigned)__shfl_xor((int)best, d, 64));
+        if ((tid & 63) == 0) sh.kred[tid >> 6] = best;
+        if (tid == 0) sh.n_cand = 0;
+        const int strange = cnt.of(kmin < W::NEG_INF || kmax > W::POS_INF);          // NaN of either sign
+#pragma unroll
+        for (int w = 0; w < T / 64; ++w) best = max(best, sh.kred[w]);
+        if (strange) {
+            top_row_again<DT, T>(A, r, sh);
+            continue;
+        }
+        // ---- the k-th largest of the threads' maxima
+        unsigned lo = W::NEG_INF + 1, hi = best;
         if (cnt.of(kmax >= lo) >= k) {
             while (lo < hi) {
                 const unsigned mid = lo + (hi - lo) / 2 + 1;
@@ -155,75 +337,67 @@ __global__ __launch_bounds__(T) void top_row_kernel(const TopArgs A) {
                 } else hi = mid - 1;
             }
         }
-        // ---- candidates
-        if (kmax >= lo)
-            each([&](unsigned key, int n) {
-                if (key >= lo) {
-                    const int p = atomicAdd(&n_cand, 1);
-                    if (p < TOP_CAP) cand[p] = composite(key, n);
-                }
-            });
+        if (lo == W::ZERO) --lo;                                                     // -0 equals 0
+        // ---- candidates, and the sum over everything below them
+        float bits_best;
+        {
+            const unsigned w = W::from(best);
+            if constexpr (DT == ELG_F32) bits_best = i2f((int)w);
+            else if constexpr (DT == ELG_BF16) bits_best = i2f((int)(w << 16));
+            else bits_best = (float)__builtin_bit_cast(_Float16, (unsigned short)w);
+        }
+        const float m = bits_best;
+        float rest[2] = {0.f, 0.f};
+        auto push = [&](float f, int n) {
+            const int p = atomicAdd(&sh.n_cand, 1);
+            if (p < TOP_CAP) sh.cand[p] = composite(order_key(f), n);
+        };
+        const int t1 = place();
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            asm volatile("" : "+v"(z[c]));
+            const unsigned top = W::highest(W::hi(W::hi(z[c][0], z[c][1]), W::hi(z[c][2], z[c][3])));
+            const bool some = __any(top >= lo);
+            if (!A.tail && !some) continue;
+            u32x4 raw;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) raw[i] = W::from(z[c][i]);
+            float v[VEC<DT>];
+            unpack<DT>(raw, v);
+            if (some) {
+                const int n0 = (t1 + c * T) * VEC<DT> - sp.shift;
+#pragma unroll
+                for (int e = 0; e < VEC<DT>; ++e)
+                    if (W::at(z[c], e) >= lo) {
+                        push(v[e], n0 + e);
+                        v[e] = ELG_NEG_INF;
+                    }
+            }
+            if (A.tail) {
+#pragma unroll
+                for (int e = 0; e < VEC<DT>; ++e) rest[e & 1] += ex2((v[e] - m) * A.c2);
+            }
+            asm volatile("" : "+v"(rest[0]), "+v"(rest[1]));
+        }
+        if (edge >= 0) {
+            if (word_key<DT>(ze) >= lo) push(ze, edge);
+            else rest[0] += ex2((ze - m) * A.c2);
+        }
         __syncthreads();
-        int found = n_cand;
-        int tie_need = 0;
-        unsigned tie_key = 0;
+        const int found = sh.n_cand;
         if (found > TOP_CAP) {
-            // the k-th largest key of all elements: count(>= lo) >= k holds throughout
-            hi = 0xFFFFFFFFu;
-            while (lo < hi) {
-                const unsigned mid = lo + (hi - lo) / 2 + 1;
-                int c = 0;
-                each([&](unsigned key, int) { c += key >= mid; });
-                int before;
-                c = cnt.scan(c, before);
-                if (c >= k) {
-                    lo = mid;
-                    if (c == k) break;
-                } else hi = mid - 1;
-            }
-            if (tid == 0) n_cand = 0;
-            __syncthreads();
-            each([&](unsigned key, int n) {
-                if (key > lo) cand[atomicAdd(&n_cand, 1)] = composite(key, n);       // fewer than k of them
-            });
-            __syncthreads();
-            found = n_cand;
-            tie_key = lo;
-            tie_need = k - found;
-        } else if (found < k) {
-            tie_key = KEY_NEG_INF;                                                   // closed nodes fill the rest
-            tie_need = k - found;
+            top_row_again<DT, T>(A, r, sh);
+            continue;
         }
-        // ---- rank by counting; composites are unique
-        for (int i = tid; i < found; i += T) {
-            const unsigned long long me = cand[i];
-            int rank = 0;
-            for (int j = 0; j < found; ++j) rank += cand[j] > me;
-            if (rank < k) win[rank] = me;
-        }
-        ties(tie_key, min(found, k), tie_need);
-        __syncthreads();
-        for (int i = tid; i < k; i += T) {
-            const unsigned long long w = win[i];
-            reinterpret_cast<elem_t<DT>*>(A.values)[r * k + i] = (elem_t<DT>)key_value((unsigned)(w >> 32));
-            A.idx[r * k + i] = (int)~(unsigned)w;
-        }
-        if (A.tail) {
-            // mass outside the winners: summed apart from the winners' own, so that a small tail keeps its digits
-            const unsigned long long last = win[k - 1];
-            const float m = key_value((unsigned)(win[0] >> 32));
-            float top = 0.f, rest = 0.f;
-            if (m > ELG_NEG_INF || m != m) {
-                for (int i = tid; i < k; i += T) top += ex2((key_value((unsigned)(win[i] >> 32)) - m) * A.c2);
-                each([&](unsigned key, int n) {
-                    if (composite(key, n) < last) rest += ex2((key_value(key) - m) * A.c2);
-                });
-            }
-            const float2 s = red.sum2(top, rest);
-            if (tid == 0) A.tail[r] = s.x + s.y > 0.f || s.x != s.x || s.y != s.y ? s.y / (s.x + s.y) : 0.f;
-        }
-        __syncthreads();                  // win, cand and n_cand are written again by the next row
+        finish_row<DT, T>(A, r, row, found, KEY_NEG_INF, found < k ? k - found : 0, rest[0] + rest[1], true, sh, cnt, red);
     }
+}
+
+// rows that no workgroup can hold
+template <int DT, int T>
+__global__ __launch_bounds__(T) void top_long_kernel(const TopArgs A) {
+    __shared__ TopShared<T> sh;
+    for (long long r = blockIdx.x; r < A.R; r += gridDim.x) top_row_again<DT, T>(A, r, sh);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
@@ -651,10 +825,10 @@ void launch_top(const TopArgs& A, hipStream_t s) {
     else if (A.V <= 2048) launch_wave<DT, 32>(A, s);
     else if (nch <= 256 * 4) launch_row<DT, 256, 4>(A, s);
     else if (nch <= 256 * 8) launch_row<DT, 256, 8>(A, s);
-    else if (nch <= 512 * 8) launch_row<DT, 512, 8>(A, s);
-    else if (nch <= 1024 * 8) launch_row<DT, 1024, 8>(A, s);
+    else if (nch <= 256 * 16) launch_row<DT, 256, 16>(A, s);
+    else if (nch <= 512 * 16) launch_row<DT, 512, 16>(A, s);
     else if (nch <= 1024 * 16) launch_row<DT, 1024, 16>(A, s);
-    else launch_row<DT, 1024, 0>(A, s);
+    else hipLaunchKernelGGL((top_long_kernel<DT, 1024>), dim3((unsigned)(A.R < 512 ? A.R : 512)), dim3(1024), 0, s, A);
 }
 
 }  // namespace
