@@ -32,13 +32,13 @@ struct DistillArgs {
     float* loss_rows;
     double* part;                         // one partial loss per workgroup, or null
     float* total;                         // the loss itself, where one workgroup sees every row; or null
+    float4* rec;                          // two a row: what a long row's loss is formed from; or null
     char* grad;                           // (R, V) packed, or null
     long long g_stride;                   // bytes
 };
 
 constexpr float TINY_MASS = 1e-36f;       // a (log a - log p_rest) below this is nothing in f32
-// The loss is formed in base 2, every difference of logits times the one rounded c2 of the exponentials, and brought to base e at its end: with
-// 1 / tau rounded apart from c2 the two would differ by 2^-24 of every difference, the same way in every row.
+// the loss is formed in base 2, like the exponentials, and brought to base e at its end
 constexpr float LN2 = 0.6931471805599453f;
 __device__ __forceinline__ float lg2(float x) { return __builtin_amdgcn_logf(x); }       // v_log_f32
 
@@ -77,28 +77,61 @@ struct Entry {
 // What a row comes down to, given its maxima and sums; the same in every thread.
 struct RowScalars {
     bool live;
-    float loss, q_scale, m, inv_S, c_rest, m_rest, G;
+    float q_scale, m, inv_S, c_rest, m_rest, G;
+    float a, S, st, sr, sd;
     // mt, mz, mr: largest teacher logit, entry's logit, other logit (-inf: none); st, sz, sr: sums of exponentials relative to each;
     // sd: sum over entries of e^((t - mt) / tau) ((t - mt) - (z - m))
-    __device__ __forceinline__ RowScalars(const DistillArgs& A, long long r, float w, float mt, float mz, float mr, float st, float sz, float sr, float sd) {
-        float a = A.tail ? A.tail[r] : 0.f;
+    __device__ __forceinline__ RowScalars(const DistillArgs& A, long long r, float w, float mt, float mz, float mr, float st_, float sz, float sr_, float sd_)
+        : st(st_), sr(sr_), sd(sd_) {
+        a = A.tail ? A.tail[r] : 0.f;
         a = a > 1.f ? 1.f : a < 0.f ? 0.f : a;
         m = fmaxf(mz, mr);
         m_rest = mr > ELG_NEG_INF ? mr : 0.f;
         const float f_top = mz > ELG_NEG_INF ? ex2((mz - m) * A.c2) : 0.f, f_rest = mr > ELG_NEG_INF ? ex2((mr - m) * A.c2) : 0.f;
-        const float S = sz * f_top + sr * f_rest;
+        S = sz * f_top + sr * f_rest;
         live = !(S <= 0.f) && !(st <= 0.f);
         inv_S = __builtin_amdgcn_rcpf(S);
         q_scale = st <= 0.f ? 0.f : (1.f - a) * __builtin_amdgcn_rcpf(st);
-        float L = sd * q_scale * A.c2;
-        if (a < 1.f) L += (1.f - a) * lg2(q_scale * S);
-        if (a > TINY_MASS) L += a * (lg2(a * S * __builtin_amdgcn_rcpf(sr)) - (m_rest - m) * A.c2);
-        loss = live ? L * (LN2 * A.tau * A.tau * w) : 0.f;
         const float cot = A.cot ? A.cot[r * A.cot_stride] : 1.f;
         G = live ? A.scale * cot * w * A.tau : 0.f;
         c_rest = live ? G * (f_rest * inv_S - (a > 0.f && sr > 0.f ? a * __builtin_amdgcn_rcpf(sr) : 0.f)) : 0.f;
+        for (float* x : {&q_scale, &m, &inv_S, &c_rest, &m_rest, &G, &S}) *x = i2f(__builtin_amdgcn_readfirstlane(f2i(*x)));
+    }
+    // what a row's loss is formed from later (S = 0: it has none)
+    __device__ __forceinline__ void record(const DistillArgs& A, long long r, float w) const {
+        A.rec[2 * r] = make_float4(live ? S : 0.f, st, sr, sd);
+        A.rec[2 * r + 1] = make_float4(a, m_rest - m, w, 0.f);
     }
 };
+
+// The losses of long rows from their records, in 64 bits: v_log_f32 is off by a half step of 1 near 1, the same way in every row, and a student
+// near its teacher has both its logarithms there.  A thread a row, away from the kernels that hold a row in registers; one partial sum a workgroup.
+__global__ __launch_bounds__(256) void distill_long_loss_kernel(const DistillArgs A) {
+    __shared__ double red[4];
+    double lacc = 0.0;
+    for (long long r = (long long)blockIdx.x * 256 + threadIdx.x; r < A.R; r += (long long)gridDim.x * 256) {
+        const float4 u = A.rec[2 * r], v = A.rec[2 * r + 1];
+        double L = 0.0;
+        if (u.x != 0.f) {
+            const double t = 1.0 / (double)A.tau, d = (double)v.x, S = (double)u.x, st = (double)u.y;
+            L = (double)u.w * (1.0 - d) / st * t;
+            if (v.x < 1.f) L += (1.0 - d) * log((1.0 - d) / st * S);
+            if (v.x > 0.f) L += d * (log(d * S / (double)u.z) - (double)v.y * t);
+            L *= (double)A.tau * (double)A.tau * (double)v.z;
+        }
+        if (A.loss_rows) A.loss_rows[r] = (float)(L * (double)A.scale);
+        lacc += L;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) lacc += __shfl_xor(lacc, d, 64);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = lacc;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const double all = (red[0] + red[1]) + (red[2] + red[3]);
+        if (A.total) A.total[0] = (float)(all * (double)A.scale);
+        else if (A.part) A.part[blockIdx.x] = all;
+    }
+}
 
 // N sums or maxima over the workgroup: one LDS exchange, one barrier; buffers alternate
 template <int W, int N>
@@ -120,6 +153,8 @@ struct BlockN {
         for (int w = 1; w < W; ++w)
 #pragma unroll
             for (int i = 0; i < N; ++i) v[i] = MAX ? fmaxf(v[i], s[w * N + i]) : v[i] + s[w * N + i];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = i2f(__builtin_amdgcn_readfirstlane(f2i(v[i])));      // the same in every lane: a scalar register
     }
 };
 
@@ -212,7 +247,7 @@ __device__ __forceinline__ void store_zero(char* grow, const Span<DT>& sp, int t
 
 // One workgroup per row, the row in registers, C chunks a thread (T C 16 bytes of it): one read, one write.
 template <int DT, int T, int C>
-__global__ __launch_bounds__(T) void distill_row_kernel(const DistillArgs A) {
+__global__ __launch_bounds__(T, 4) void distill_row_kernel(const DistillArgs A) {
     static_assert(T >= ELG_TOP_MAX_K, "one entry per thread");
     constexpr int W = T / 64;
     __shared__ unsigned bits[T * C * VEC<DT> / 32];
@@ -222,7 +257,6 @@ __global__ __launch_bounds__(T) void distill_row_kernel(const DistillArgs A) {
     const int tid = threadIdx.x, V = A.V, k = A.k;
     BlockN<W, 3> bmax(mred);
     BlockN<W, 4> bsum(sred);
-    double lacc = 0.0;
     for (int i = tid; i < T * C * VEC<DT> / 32; i += T) bits[i] = 0u;
     if (tid < ELG_TOP_MAX_K) eidx[tid] = -2;
     __syncthreads();
@@ -233,7 +267,7 @@ __global__ __launch_bounds__(T) void distill_row_kernel(const DistillArgs A) {
         const float w = A.weight ? A.weight[r] : 1.f;
         const int edge = sp.edge(tid);
         if (w == 0.f) {                   // the row is not looked at
-            if (tid == 0 && A.loss_rows) A.loss_rows[r] = 0.f;
+            if (tid == 0 && A.rec) A.rec[2 * r] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (grow) store_zero<DT>(grow, sp, tid, T, sp.c_hi, edge);
             continue;
         }
@@ -281,10 +315,7 @@ __global__ __launch_bounds__(T) void distill_row_kernel(const DistillArgs A) {
         if (en.i >= 0) bits[(en.i + sp.shift) >> 5] = 0u;              // clean for the next row
         bsum.template run<false>(sm);
         const RowScalars s(A, r, w, mx[0], mx[1], mx[2], sm[0], sm[1], sm[2], sm[3]);
-        if (tid == 0) {
-            if (A.loss_rows) A.loss_rows[r] = s.loss * A.scale;
-            lacc += (double)s.loss;
-        }
+        if (tid == 0 && A.rec) s.record(A, r, w);
         if (grow) {
             store_rest<DT, C>(grow, sp, place(), T, sp.c_hi, zr, edge, ze, s, A.c2);
             __syncthreads();
@@ -292,7 +323,6 @@ __global__ __launch_bounds__(T) void distill_row_kernel(const DistillArgs A) {
         }
         __syncthreads();                  // the entries' LDS is written again by the next row
     }
-    if (A.part && tid == 0) A.part[blockIdx.x] = lacc;
 }
 
 // Few long rows, or rows beyond what a workgroup can hold: a row is split into segments of SEG_T SEG_C chunks, a workgroup each.  The first
@@ -371,10 +401,7 @@ __global__ __launch_bounds__(SEG_T) void distill_join_kernel(const DistillArgs A
     const int c_end = min(sp.c_hi, c_lo + SEG_T * SEG_C), edge = seg == grid_segs - 1 ? sp.edge(tid) : -1;
     const float w = A.weight ? A.weight[r] : 1.f;
     if (w == 0.f) {
-        if (tid == 0 && seg == 0) {
-            if (A.loss_rows) A.loss_rows[r] = 0.f;
-            if (A.part) A.part[r] = 0.0;
-        }
+        if (tid == 0 && seg == 0 && A.rec) A.rec[2 * r] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (grow) store_zero<DT>(grow, sp, c_lo + tid, SEG_T, c_end, edge);
         return;
     }
@@ -406,10 +433,7 @@ __global__ __launch_bounds__(SEG_T) void distill_join_kernel(const DistillArgs A
     if (tid < k) ee[tid] = mine;
     bsum.template run<false>(sm);
     const RowScalars s(A, r, w, mx[0], mx[1], mx[2], sm[0], sm[1], sm[2], sm[3]);
-    if (tid == 0 && seg == 0) {
-        if (A.loss_rows) A.loss_rows[r] = s.loss * A.scale;
-        if (A.part) A.part[r] = (double)s.loss;
-    }
+    if (tid == 0 && seg == 0 && A.rec) s.record(A, r, w);
     if (!grow) return;
     store_rest<DT, SEG_C>(grow, sp, c_lo + tid, SEG_T, c_end, zr, edge, ze, s, A.c2);
     __syncthreads();
@@ -599,7 +623,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistillArgs A)
         const float q_scale = st <= 0.f ? 0.f : (1.f - a) * __builtin_amdgcn_rcpf(st);
         const bool live = x.w != 0.f && !(S <= 0.f) && !(st <= 0.f);
         if (A.loss_rows || A.part || A.total) {
-            float L = gsum<G>(sd) * q_scale * A.c2;
+            float L = (gsum<G>(sd) * q_scale) * A.c2;
             if (a < 1.f) L += (1.f - a) * lg2(q_scale * S);
             if (a > TINY_MASS) L += a * (lg2(a * S * inv_sr) - (m_rest - m) * A.c2);
             L = live ? L * (LN2 * A.tau * A.tau * x.w) : 0.f;
@@ -672,20 +696,24 @@ struct Plan {
     int lanes;                            // of a short row; 0: a workgroup or more
     bool split;
     int segs;
-    bool one;                             // so few short rows that one workgroup forms their total: a launch and the scratch saved
-    long long parts;                      // workgroups and, unless `one`, partial losses
+    long long grid;                       // workgroups of the kernel that sees the rows
+    long long parts;                      // partial losses; 1: the loss itself is written, no scratch for them
     Plan(long long R, long long V, int type) {
         const int vec = type == ELG_F32 ? 4 : 8;
-        // rows that no workgroup can hold, or so few long ones that most of the chip would idle: measured, 6 rows of 100003 f32: 142 us a
-        // workgroup each, 24 us split; 256 rows of 32000 bf16: 16 and 19 us
+        // rows that no workgroup can hold, or so few long ones that most of the chip would idle: 6 rows of 100003 f32, the gradient in 35 us and
+        // more by a workgroup each, in 10 us split
         lanes = V <= 256 ? 16 : V <= 2048 ? 64 : 0;
         split = !lanes && (V > 1024 * 16 * vec || (R <= 64 && V > 1024 * vec));
         segs = split ? (int)((V + vec - 1 + SEG_T * SEG_C * vec - 1) / (SEG_T * SEG_C * vec)) : 0;     // a row may start inside its first 16 bytes
         const long long rows_wg = lanes == 16 ? 16 : lanes == 64 ? 4 : 1, want = (R + rows_wg - 1) / rows_wg;
-        one = lanes && want <= 8;
-        parts = split ? R : want < MAX_GRID ? want : MAX_GRID;
+        grid = want < MAX_GRID ? want : MAX_GRID;
+        // so few short rows that one workgroup forms their total: a launch and the scratch saved.  Long rows: a thread a row
+        parts = lanes ? (want <= 8 ? 1 : grid) : R <= 1024 ? 1 : (R + 255) / 256 < 256 ? (R + 255) / 256 : 256;
     }
-    long long bytes(long long R) const { return one ? 0 : 8 * parts + 8 * R * segs; }
+    // partial losses | records of long rows | segments of split ones
+    long long rec_at() const { return parts > 1 ? 8 * ((parts + 1) / 2 * 2) : 0; }
+    long long segs_at(long long R) const { return rec_at() + (lanes ? 0 : 32 * R); }
+    long long bytes(long long R) const { return segs_at(R) + 8 * R * segs; }
 };
 
 template <int DT, int T, int C>
@@ -697,7 +725,7 @@ void launch_row(const DistillArgs& A, int grid, hipStream_t s) {
 // workgroup or several.
 template <int DT>
 void launch(const DistillArgs& A, const Plan& P, float2* parts, hipStream_t s) {
-    const int V = A.V, k = A.k, grid = A.total ? 1 : (int)P.parts;
+    const int V = A.V, k = A.k, grid = P.lanes && A.total ? 1 : (int)P.grid;
     // chunks a row can span: its own and, unless every row starts on 16 bytes, what the first line holds in front of it
     const bool aligned = !((uintptr_t)A.z & 15) && !(A.z_stride & 15);
     const int nch = (V + (aligned ? 0 : VEC<DT> - 1) + VEC<DT> - 1) / VEC<DT>;
@@ -715,8 +743,8 @@ void launch(const DistillArgs& A, const Plan& P, float2* parts, hipStream_t s) {
         hipLaunchKernelGGL((distill_join_kernel<DT>), dim3((unsigned)(A.R * grad_segs)), dim3(SEG_T), 0, s, A, parts, P.segs, grad_segs);
     } else if (nch <= 256 * 4) launch_row<DT, 256, 4>(A, grid, s);
     else if (nch <= 256 * 8) launch_row<DT, 256, 8>(A, grid, s);
-    else if (nch <= 512 * 8) launch_row<DT, 512, 8>(A, grid, s);
-    else if (nch <= 1024 * 8) launch_row<DT, 1024, 8>(A, grid, s);
+    else if (nch <= 256 * 16) launch_row<DT, 256, 16>(A, grid, s);
+    else if (nch <= 512 * 16) launch_row<DT, 512, 16>(A, grid, s);
     else if (nch <= 1024 * 16) launch_row<DT, 1024, 16>(A, grid, s);
     else launch_row<DT, 1024, 17>(A, grid, s);
 }
@@ -744,25 +772,31 @@ extern "C" int elg_distill_loss_grad(const void* z, int64_t z_stride, int type, 
     if (!loss_rows && !loss_total && !grad) return fail(ELG_EINVAL, "distill: nothing to compute");
     if (R > 0 && (!z || !top_values || !top_idx)) return fail(ELG_EINVAL, "distill: null buffer");
     const Plan P(R, V, type);
-    if (R > 0 && P.bytes(R) > 0 && (loss_total || P.split) && (!ws || ws_bytes < P.bytes(R))) return fail(ELG_EINVAL, "distill: needs elg_distill_ws_bytes() of scratch");
+    const bool want_loss = loss_rows || loss_total, scratch = P.split || (P.lanes ? loss_total && P.parts > 1 : want_loss);
+    if (R > 0 && scratch && (!ws || ws_bytes < P.bytes(R))) return fail(ELG_EINVAL, "distill: needs elg_distill_ws_bytes() of scratch");
     if (R * (P.segs + 1) > 0x7FFFFFFF) return fail(ELG_EINVAL, "distill: too many long rows for one call");
     if (R == 0 && !loss_total) return ELG_OK;
     const int es = type == ELG_F32 ? 4 : 2;
-    if (((uintptr_t)z | (uintptr_t)grad) % es || (uintptr_t)top_values % (top_type == ELG_F32 ? 4 : 2) || (uintptr_t)top_idx % (idx_wide ? 8 : 4) || (uintptr_t)ws % 8)
+    if (((uintptr_t)z | (uintptr_t)grad) % es || (uintptr_t)top_values % (top_type == ELG_F32 ? 4 : 2) || (uintptr_t)top_idx % (idx_wide ? 8 : 4) || (uintptr_t)ws % 16)
         return fail(ELG_EINVAL, "distill: misaligned buffer");
     DistillArgs A;
     A.z = (const char*)z; A.z_stride = z_stride * es; A.R = R; A.V = (int)V; A.k = k;
     A.tv = top_values; A.ti = top_idx; A.tv_type = top_type; A.ti_wide = idx_wide != 0;
     A.tail = tail; A.weight = weight; A.cot = cot; A.cot_stride = cot_stride;
     A.tau = temperature; A.c2 = LOG2E / temperature; A.scale = scale;
-    A.loss_rows = loss_rows; A.part = loss_total && !P.one ? (double*)ws : nullptr; A.total = P.one ? loss_total : nullptr;
+    A.loss_rows = loss_rows;
+    A.part = loss_total && P.parts > 1 ? (double*)ws : nullptr;
+    A.total = loss_total && P.parts == 1 ? loss_total : nullptr;
+    A.rec = want_loss && !P.lanes && R > 0 ? reinterpret_cast<float4*>((char*)ws + P.rec_at()) : nullptr;
     A.grad = (char*)grad; A.g_stride = V * es;
     (void)hipGetLastError();
     hipStream_t st = (hipStream_t)stream;
     if (R > 0) {
-        float2* parts = reinterpret_cast<float2*>((char*)ws + 8 * P.parts);
+        float2* parts = reinterpret_cast<float2*>((char*)ws + P.segs_at(R));
         type == ELG_F32 ? launch<ELG_F32>(A, P, parts, st) : type == ELG_BF16 ? launch<ELG_BF16>(A, P, parts, st) : launch<ELG_F16>(A, P, parts, st);
+        if (A.rec) hipLaunchKernelGGL(distill_long_loss_kernel, dim3((unsigned)(P.parts > 1 ? P.parts : R > 256 ? (A.total ? 1 : 4) : 1)), dim3(256), 0, st, A);
     }
-    if (loss_total && !(P.one && R > 0)) hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(256), 0, st, (const double*)ws, R > 0 ? (int)P.parts : 0, scale, loss_total);
+    if (loss_total && (A.part || R == 0))
+        hipLaunchKernelGGL(distill_total_kernel, dim3(1), dim3(256), 0, st, (const double*)ws, R > 0 ? (int)P.parts : 0, scale, loss_total);
     return launch_status("distill");
 }

@@ -13,6 +13,7 @@
 namespace elg {
 namespace {
 
+constexpr int WAVE_CAP = 256;             // candidates of a wave
 constexpr int TOP_CAP = 1024;             // candidates kept in LDS; more of them: the bisection over the whole row
 
 struct TopArgs {
@@ -115,8 +116,10 @@ __device__ __forceinline__ unsigned word_key(float f) {
 
 template <int T>
 struct TopShared {
-    unsigned long long cand[TOP_CAP];
-    unsigned long long win[ELG_TOP_MAX_K];
+    unsigned long long found[T / 64][WAVE_CAP];       // as a wave finds them
+    int n_found[T / 64];
+    __attribute__((aligned(16))) unsigned long long cand[TOP_CAP + 8];       // all of them, in any order
+    unsigned long long win[TOP_CAP];      // in order
     float fred[2 * 2 * (T / 64)];
     int cred[2 * (T / 64)];
     unsigned kred[2 * (T / 64)];
@@ -151,17 +154,25 @@ __device__ __forceinline__ void take_ties(const void* row, int V, unsigned key, 
     }
 }
 
-// the candidates in order into win (the first k of them); what the others of them and the rest weigh
+// the candidates in order into win, the first k of it written out; what the others of them and the rest weigh
 template <int DT, int T>
 __device__ __forceinline__ void finish_row(const TopArgs& A, long long r, const void* row, int found, unsigned tie_key, int tie_need, float rest, bool rest_known,
                                            TopShared<T>& sh, Count<T>& cnt, BlockRed<T / 64>& red) {
     const int tid = threadIdx.x, k = A.k;
-    // rank by counting; composites are unique
+    // rank by counting; composites are unique, and none is 0
+    if (tid < 8) sh.cand[found + tid] = 0ull;
+    __syncthreads();
     for (int i = tid; i < found; i += T) {
         const unsigned long long me = sh.cand[i];
         int rank = 0;
-        for (int j = 0; j < found; ++j) rank += sh.cand[j] > me;
-        if (rank < k) sh.win[rank] = me;
+        for (int j = 0; j < found; j += 8) {          // eight at a time: one LDS latency, not eight
+            ulonglong2 o[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) o[u] = *reinterpret_cast<const ulonglong2*>(sh.cand + j + 2 * u);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) rank += (o[u].x > me) + (o[u].y > me);
+        }
+        sh.win[rank] = me;
     }
     take_ties<DT, T>(row, A.V, tie_key, min(found, k), tie_need, sh.win, cnt);
     __syncthreads();
@@ -179,8 +190,7 @@ __device__ __forceinline__ void finish_row(const TopArgs& A, long long r, const 
         else {
             for (int i = tid; i < k; i += T) top += ex2((key_value((unsigned)(sh.win[i] >> 32)) - m) * A.c2);
             if (rest_known) {
-                for (int i = tid; i < found; i += T)
-                    if (sh.cand[i] < last) rest += ex2((key_value((unsigned)(sh.cand[i] >> 32)) - m) * A.c2);
+                for (int i = k + tid; i < found; i += T) rest += ex2((key_value((unsigned)(sh.win[i] >> 32)) - m) * A.c2);
             } else {
                 const int shift = shift_of<DT>(row), nch = (shift + A.V + VEC<DT> - 1) / VEC<DT>;
                 rest = 0.f;
@@ -317,7 +327,6 @@ __global__ __launch_bounds__(T, 4) void top_row_kernel(const TopArgs A) {
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) best = max(best, (unsigned)__shfl_xor((int)best, d, 64));
         if ((tid & 63) == 0) sh.kred[tid >> 6] = best;
-        if (tid == 0) sh.n_cand = 0;
         const int strange = cnt.of(kmin < W::NEG_INF || kmax > W::POS_INF);          // NaN of either sign
 #pragma unroll
         for (int w = 0; w < T / 64; ++w) best = max(best, sh.kred[w]);
@@ -325,7 +334,7 @@ __global__ __launch_bounds__(T, 4) void top_row_kernel(const TopArgs A) {
             top_row_again<DT, T>(A, r, sh);
             continue;
         }
-        // ---- the k-th largest of the threads' maxima
+        // ---- the k-th largest of the threads' maxima, or a little less: a few candidates more cost less than the steps that would spare them
         unsigned lo = W::NEG_INF + 1, hi = best;
         if (cnt.of(kmax >= lo) >= k) {
             while (lo < hi) {
@@ -333,7 +342,7 @@ __global__ __launch_bounds__(T, 4) void top_row_kernel(const TopArgs A) {
                 const int c = cnt.of(kmax >= mid);
                 if (c >= k) {
                     lo = mid;
-                    if (c == k) break;
+                    if (c <= k + k / 8 + 4) break;
                 } else hi = mid - 1;
             }
         }
@@ -348,9 +357,13 @@ __global__ __launch_bounds__(T, 4) void top_row_kernel(const TopArgs A) {
         }
         const float m = bits_best;
         float rest[2] = {0.f, 0.f};
-        auto push = [&](float f, int n) {
-            const int p = atomicAdd(&sh.n_cand, 1);
-            if (p < TOP_CAP) sh.cand[p] = composite(order_key(f), n);
+        // (a wave keeps its own list: no atomics, no waiting)
+        int n_mine = 0;
+        auto push = [&](bool hit, float f, int n) {
+            const unsigned long long mask = __ballot(hit);
+            const int p = n_mine + lanes_below(mask);
+            if (hit && p < WAVE_CAP) sh.found[tid >> 6][p] = composite(order_key(f), n);
+            n_mine += __popcll(mask);
         };
         const int t1 = place();
 #pragma unroll
@@ -367,11 +380,11 @@ __global__ __launch_bounds__(T, 4) void top_row_kernel(const TopArgs A) {
             if (some) {
                 const int n0 = (t1 + c * T) * VEC<DT> - sp.shift;
 #pragma unroll
-                for (int e = 0; e < VEC<DT>; ++e)
-                    if (W::at(z[c], e) >= lo) {
-                        push(v[e], n0 + e);
-                        v[e] = ELG_NEG_INF;
-                    }
+                for (int e = 0; e < VEC<DT>; ++e) {
+                    const bool hit = W::at(z[c], e) >= lo;
+                    push(hit, v[e], n0 + e);
+                    v[e] = hit ? ELG_NEG_INF : v[e];
+                }
             }
             if (A.tail) {
 #pragma unroll
@@ -379,16 +392,27 @@ __global__ __launch_bounds__(T, 4) void top_row_kernel(const TopArgs A) {
             }
             asm volatile("" : "+v"(rest[0]), "+v"(rest[1]));
         }
-        if (edge >= 0) {
-            if (word_key<DT>(ze) >= lo) push(ze, edge);
-            else rest[0] += ex2((ze - m) * A.c2);
+        {
+            const bool hit = edge >= 0 && word_key<DT>(ze) >= lo;
+            push(hit, ze, edge);
+            if (edge >= 0 && !hit) rest[0] += ex2((ze - m) * A.c2);
         }
+        if ((tid & 63) == 0) sh.n_found[tid >> 6] = n_mine;
         __syncthreads();
-        const int found = sh.n_cand;
-        if (found > TOP_CAP) {
+        int found = 0, at = 0;
+        bool over = false;
+#pragma unroll
+        for (int w = 0; w < T / 64; ++w) {
+            const int n = sh.n_found[w];
+            if (w < (tid >> 6)) at += n;
+            found += n;
+            over = over || n > WAVE_CAP;
+        }
+        if (found > TOP_CAP || over) {
             top_row_again<DT, T>(A, r, sh);
             continue;
         }
+        for (int i = tid & 63; i < n_mine; i += 64) sh.cand[at + i] = sh.found[tid >> 6][i];
         finish_row<DT, T>(A, r, row, found, KEY_NEG_INF, found < k ? k - found : 0, rest[0] + rest[1], true, sh, cnt, red);
     }
 }
@@ -707,7 +731,7 @@ __global__ __launch_bounds__(256) void top_wave_kernel(const TopArgs A) {
                 const int c = groups(mid);
                 if (c >= k) {
                     lo = mid;
-                    if (c == k) break;
+                    if (c <= k + k / 8 + 4) break;
                 } else hi = mid - 1;
             }
         int found = z.count(lo), ties = 0;

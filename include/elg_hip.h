@@ -496,7 +496,7 @@ int elg_top_logits(const void* z, int64_t z_stride, int type, int64_t R, int64_t
  *   loss_rows (R) or NULL  = scale L_r
  *   loss_total (1) or NULL = scale sum_r L_r, added in 64 bits in an order fixed by the sizes
  *   grad (R,V) packed, of `type`, or NULL = scale cot_r dL_r/dz; cot: NULL (1), one number (cot_stride 0) or one per row (1)
- * ws: elg_distill_ws_bytes() bytes, 8-byte aligned; 0 bytes, and rows of up to 2048 logits without
+ * ws: elg_distill_ws_bytes() bytes, 16-byte aligned; 0 bytes, and rows of up to 2048 logits without
  * loss_total: may be NULL. */
 int64_t elg_distill_ws_bytes(int64_t R, int64_t V, int type);
 int elg_distill_loss_grad(const void* z, int64_t z_stride, int type, int64_t R, int64_t V, const void* top_values, int top_type,
