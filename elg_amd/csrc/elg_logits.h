@@ -97,24 +97,8 @@ __device__ __forceinline__ u32x4 load_chunk(const void* row, int shift, int V, i
     }
     return r;
 }
-// the bits of -inf / of 0, as load_chunk's pad
+// the bits of -inf, as load_chunk's pad
 template <int DT> constexpr unsigned PAD_NEG_INF = DT == ELG_F32 ? 0xFF800000u : DT == ELG_BF16 ? 0xFF80FF80u : 0xFC00FC00u;
-
-// chunk c of a row written back; only positions inside the row are touched
-template <int DT>
-__device__ __forceinline__ void store_chunk(void* row, int shift, int V, int c, const float (&v)[VEC<DT>]) {
-    const int n0 = c * VEC<DT> - shift;
-    elem_t<DT>* p = reinterpret_cast<elem_t<DT>*>(row);
-    if (n0 >= 0 && n0 + VEC<DT> <= V && !((uintptr_t)(p + n0) & 15)) {
-        *reinterpret_cast<u32x4*>(p + n0) = pack<DT>(v);
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < VEC<DT>; ++e) {
-        const int n = n0 + e;
-        if (n >= 0 && n < V) p[n] = (elem_t<DT>)v[e];
-    }
-}
 
 // The same row as whole chunks [c_lo, c_hi) and the few elements in front of and behind them: loops over whole chunks need no per-chunk
 // case distinction, and thread t < 2 VEC takes the single element edge(t) besides.  For rows of at least 2 VEC elements.
@@ -141,7 +125,7 @@ struct Span {
     __device__ __forceinline__ u32x4 chunk(int c) const { return *reinterpret_cast<const u32x4*>(base + 16u * (unsigned)c); }
 };
 
-// block-wide sum / max: one LDS exchange and one barrier each; `slot` alternates between two buffers so that a wave may enter the next
+// block-wide sums: one LDS exchange and one barrier; `slot` alternates between two buffers so that a wave may enter the next
 // reduction while another still reads this one.  Every thread gets the result, added in wave order (the same bits in every run).
 template <int W>
 struct BlockRed {
@@ -158,18 +142,6 @@ struct BlockRed {
         float2 r = make_float2(s[0], s[1]);
 #pragma unroll
         for (int w = 1; w < W; ++w) { r.x += s[2 * w]; r.y += s[2 * w + 1]; }
-        return r;
-    }
-    __device__ __forceinline__ float2 max2(float a, float b) {
-        a = wave_max(a);
-        b = wave_max(b);
-        float* s = buf + flip * 2 * W;
-        flip ^= 1;
-        if ((threadIdx.x & 63) == 0) { s[2 * (threadIdx.x >> 6)] = a; s[2 * (threadIdx.x >> 6) + 1] = b; }
-        __syncthreads();
-        float2 r = make_float2(s[0], s[1]);
-#pragma unroll
-        for (int w = 1; w < W; ++w) { r.x = fmaxf(r.x, s[2 * w]); r.y = fmaxf(r.y, s[2 * w + 1]); }
         return r;
     }
 };

@@ -865,7 +865,7 @@ extern "C" int elg_top_logits(const void* z, int64_t z_stride, int type, int64_t
     if (type != ELG_F32 && type != ELG_BF16 && type != ELG_F16) return fail(ELG_EINVAL, "top_logits: unknown element type");
     if (R < 0 || V <= 0 || V > ELG_ROW_MAX_V) return fail(ELG_EINVAL, "top_logits: rows of 1 .. 2^24 logits");
     if (k < 1 || k > ELG_TOP_MAX_K || k > V) return fail(ELG_EINVAL, "top_logits: 1 <= k <= min(V, 256)");
-    if (!(temperature > 0.f) || temperature > 3.4e38f) return fail(ELG_EINVAL, "top_logits: the temperature must be positive and finite");
+    if (!(temperature >= 1e-15f && temperature <= 1e15f)) return fail(ELG_EINVAL, "top_logits: the temperature must lie in 1e-15 .. 1e15");
     if (R == 0) return ELG_OK;
     if (!z || !values || !idx) return fail(ELG_EINVAL, "top_logits: null buffer");
     const int es = type == ELG_F32 ? 4 : 2;

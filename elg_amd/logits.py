@@ -67,8 +67,8 @@ def _rows(t: torch.Tensor, what: str) -> torch.Tensor:
 
 def _temperature(t: float) -> float:
     t = float(t)
-    if not 0.0 < t <= 3.0e38:
-        raise ValueError(f"the temperature must be positive and finite, got {t}")
+    if not 1e-15 <= t <= 1e15:
+        raise ValueError(f"the temperature must lie in 1e-15 .. 1e15, got {t}")
     return t
 
 

@@ -479,7 +479,7 @@ int64_t elg_decoder_bwd_ws_floats(int32_t B, int64_t R, int32_t N1);
  * Row operators over node logits / probabilities: what one policy leaves behind for another (its best logits), the loss that
  * teaches the other on them, and the check of choices the other has drafted.  Rows as elg_rollout_fwd dumps them (full_probs:
  * closed nodes -inf / 0), or anybody's rows of 1 .. ELG_ROW_MAX_V entries.  No 16-byte alignment is needed; strides are in
- * elements.  `type`: ELG_F32 / ELG_BF16 / ELG_F16.  Nothing is kept between calls; workspaces are the call's own.
+ * elements; temperatures lie in 1e-15 .. 1e15.  `type`: ELG_F32 / ELG_BF16 / ELG_F16.  Nothing is kept between calls; workspaces are the call's own.
  * ------------------------------------------------------------------------------------------------------------------------- */
 
 /* The k best logits of each row z[r z_stride + n], n < V: values (R,k) of the same type, idx (R,k), best first.  Equal logits: the

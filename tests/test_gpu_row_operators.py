@@ -203,6 +203,41 @@ def test_distill_sizes(V, k, dtype):
         check_distill(z, tv, ti, a, tau, None, dtype)
 
 
+@pytest.mark.parametrize("dtype,V", [("float32", 4099), ("float32", 8191), ("float32", 12001), ("float32", 16384), ("float32", 30011), ("float32", 65536),
+                                     ("float32", 65533), ("bfloat16", 9001), ("bfloat16", 16001), ("bfloat16", 32768), ("float16", 60001),
+                                     ("bfloat16", 131072), ("float16", 131071)])
+def test_distill_long_rows_by_the_dozen(dtype, V):
+    """Enough long rows for a workgroup each: every size of workgroup, rows that start at every alignment, weights and repeated nodes."""
+    R, k = 70, 100
+    z = rows("closed", R, V, V, TYPES[dtype])
+    z[:, 5] = 2.0
+    tv, ti, a = teacher_of(z, k, 7)
+    ti[::3, 40:44] = ti[::3, :1]
+    ti[1::3, -3:] = -1
+    tv = torch.where(torch.isfinite(tv), tv, torch.full_like(tv, -np.inf))
+    open_ = torch.isfinite(z.gather(1, ti.clamp(0, V - 1).long())) & (ti >= 0)
+    tv = torch.where(open_, tv, torch.full_like(tv, -np.inf))
+    w = torch.ones(R)
+    w[4::9] = 0.0
+    d = [t.to(DEV) for t in (z, tv, ti, a, w)]
+    loss, grad = lg().distill_loss_grad(d[0], d[1], d[2], tail=d[3], weight=d[4], reduction="none")
+    some = [0, 1, 2, 4, 33, 68, 69]
+    compare(loss[some], grad[some], z[some], tv[some], ti[some], a[some], 1.0, w[some], 1.0, dtype)
+    # the same rows a few at a time go another way
+    for at in range(0, R, 35):
+        l2, g2 = lg().distill_loss_grad(*(t[at:at + 35] for t in d[:3]), tail=d[3][at:at + 35], weight=d[4][at:at + 35], reduction="none")
+        assert torch.allclose(l2, loss[at:at + 35], rtol=1e-5, atol=1e-6)
+        assert (g2.double() - grad[at:at + 35].double()).norm() <= (2 * ro.HALF_STEP[dtype] + 1e-6) * g2.double().norm()
+    mean, gm = lg().distill_loss_grad(d[0], d[1], d[2], tail=d[3], weight=d[4])
+    assert mean.item() == pytest.approx(loss.double().mean().item(), rel=1e-6)
+    # a strided view: rows and gradient lie differently in memory
+    wide = torch.zeros(R, V + 3, dtype=TYPES[dtype], device=DEV)
+    wide[:, 1:V + 1] = d[0]
+    l3, g3 = lg().distill_loss_grad(wide[:, 1:V + 1], d[1], d[2], tail=d[3], weight=d[4], reduction="none")
+    compare(l3[some], g3[some], z[some], tv[some], ti[some], a[some], 1.0, w[some], 1.0, dtype)
+    assert torch.allclose(l3, loss, rtol=1e-5, atol=1e-6)
+
+
 @pytest.mark.parametrize("V,k", [(101, 40), (500, 40), (1500, 64), (3000, 100), (20011, 256)])
 @pytest.mark.parametrize("kind", ["spread", "lowest", "empty", "ties"])
 def test_distill_values_and_weights(V, k, kind):
@@ -249,6 +284,16 @@ def test_distill_mass_on_a_closed_node_and_an_empty_rest():
     np.testing.assert_allclose(grad.cpu().numpy(), ref, atol=1e-6)
     total = lg().distill_loss(z.to(DEV), tv.to(DEV), ti.to(DEV), tail=a.to(DEV))
     assert total.item() == np.inf
+
+
+@pytest.mark.parametrize("V", [50, 700, 3001, 40001])
+def test_distill_when_the_entries_hold_nothing(V):
+    """tail = 1: the entries' masses are 0, also where the student has closed one of their nodes; tail above 1 is taken as 1, below 0 as 0."""
+    z = rows("plain", 4, V, 5)
+    z[0, 3] = -np.inf
+    tv, ti = torch.zeros(4, 10), torch.arange(10).int().expand(4, 10).contiguous()
+    for a in (torch.ones(4), torch.tensor([1.0, 1.5, -0.25, 0.0])):
+        check_distill(z if a.min() == 1 else z.masked_fill(torch.isinf(z), -9.0), tv, ti, a, 1.3, None, "float32")
 
 
 @pytest.mark.parametrize("V", [40, 900, 5000])
