@@ -284,6 +284,9 @@ __device__ __noinline__ void top_row_again(const TopArgs& A, long long r, TopSha
 
 // One workgroup per row, the row in registers as order keys, C chunks a thread.  One pass for the threads' maxima, one that gathers the
 // candidates and sums the exponentials of everything below the bound.
+// 512 x 131072 bf16, the best 128: 84 us where its bytes take 28.  A row of 256 KB fills a CU's registers, so each CU works its two rows off one
+// after the other, and between loading them stand the maxima (two 16-bit keys to an operation), the bound's bisection and the ranking, with
+// nothing in flight behind them.  The candidates ranked eight at a time, 112 -> 90 us; keys formed in place of floats, 120 -> 112 us.
 template <int DT, int T, int C>
 __global__ __launch_bounds__(T, 4) void top_row_kernel(const TopArgs A) {
     using W = WordKey<DT>;
@@ -417,7 +420,7 @@ __global__ __launch_bounds__(T, 4) void top_row_kernel(const TopArgs A) {
     }
 }
 
-// rows that no workgroup can hold
+// rows that no workgroup can hold: read twice or more, the keys formed anew each time
 template <int DT, int T>
 __global__ __launch_bounds__(T) void top_long_kernel(const TopArgs A) {
     __shared__ TopShared<T> sh;
@@ -527,7 +530,9 @@ __device__ __forceinline__ void across(K (&x)[NE], bool up) {
 
 constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_MIRROR4 = 0x1B, DPP_MIRROR8 = 0x141;
 
-// 8 rows to a wave, 4 waves to a workgroup (2 where 4 would need over 64 KB of LDS); waves never wait for each other.  LDS turns the lanes' runs of the order into the rows' packed output.
+// 8 rows to a wave, 4 waves to a workgroup (2 where 4 would need over 64 KB of LDS); waves never wait for each other.  LDS turns the lanes'
+// runs of the order into the rows' packed output.
+// 896000 rows of 101 f32, the best 40 and the tail: 217 us where its bytes take 137 (3.0 TB/s); the sort's exchanges bound it, not memory.
 template <int DT, int NE>
 __global__ __launch_bounds__(256, NE == 32 ? 3 : 4) void top_sort_kernel(const TopArgs A) {
     using K = typename KeyOf<DT>::K;
@@ -603,9 +608,11 @@ void launch_sort(const TopArgs& A, hipStream_t s) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------
-// Rows of 257 to 2048 logits: a wave to a row, lane l holding the nodes i 64 + l.  The same selection as a workgroup's below, with counts by
+// Rows of 257 to 2048 logits: a wave to a row, lane l holding the nodes i 64 + l.  The same selection as a workgroup's, with counts by
 // ballot: a bound from the maxima of groups of NE / 4 nodes, the few candidates above it compacted through LDS, then sorted with one, two or
 // four to a lane.
+// 8000 rows of 1001 f16, the best 63 and the tail: 27 us where its bytes take 4.  All 8000 waves are resident at once, and 1280 vector and 680
+// scalar instructions a row keep the vector units busy two thirds of that time.
 template <int NE>
 struct WaveRow {
     unsigned key[NE];

@@ -136,6 +136,7 @@ __device__ __forceinline__ int pick_in_wave(const double (&r)[N], double before,
 
 // Rows of up to 64 NE probabilities: a wave to a sequence, lane l holding the nodes i 64 + l.  The sum of each run of 64 is formed once; only
 // the run in which the draw falls is scanned.
+// 6400 sequences of 8 drafts over 101 nodes: 7.4 us; one step of 100 sequences 4.4 us, a launch with a chain of four dependent reads in it.
 template <int DT, int NE>
 __global__ __launch_bounds__(256) void verify_wave_kernel(const VerifyArgs A, long long B) {
     const int lane = threadIdx.x & 63;
@@ -192,6 +193,8 @@ __global__ __launch_bounds__(256) void verify_wave_kernel(const VerifyArgs A, lo
 }
 
 // Longer rows, in segments of RUNS runs of 64 chunks, four runs to a wave of a workgroup.
+// 48 sequences over 131072 probabilities in bf16 (25 MB of two rows each): 11 us for the segments' sums, 10 us for the pick, where the bytes take
+// 5.3.  The sums convert every probability to 64 bits; the pick waits for the acceptance, the segments, a segment and a run, one after the other.
 constexpr int RUNS = 16;
 
 // the sums of a segment's runs, of what is drawn from (x) and of the target's own row (y), into LDS
