@@ -184,10 +184,13 @@ __device__ __forceinline__ float dot4(const float4 a, const float4 b, float acc)
 // Euclidean distance exactly as a plain fp32 evaluation: sqrt(dx*dx + dy*dy), every op rounded once
 // (no fma contraction) -- CVRPEnv.py:148 / :261.
 __device__ __forceinline__ float dist2d(float ax, float ay, float bx, float by) {
-    float dx = __fsub_rn(ax, bx), dy = __fsub_rn(ay, by);
+    // the _rn intrinsics are ordinary operators to this toolchain, and a product and a sum of them become one fma unless that is ruled out here
+#pragma clang fp contract(off)
+    float dx = ax - bx, dy = ay - by;
     // sqrtf, not __fsqrt_rn: this toolchain lowers __fsqrt_rn to the bare v_sqrt_f32 (1 ulp), sqrtf to the correctly rounded
     // sequence -- and a 1-ulp distance reorders near-equidistant neighbours (a different k-NN set than the reference's)
-    return sqrtf(__fadd_rn(__fmul_rn(dx, dx), __fmul_rn(dy, dy)));
+    const float xx = dx * dx, yy = dy * dy;
+    return sqrtf(xx + yy);
 }
 
 // Philox-4x32-10 counter RNG: one uniform in [0,1) per (seed, trajectory, step).

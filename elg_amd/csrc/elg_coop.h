@@ -175,7 +175,12 @@ __device__ __forceinline__ void co_local_tail(const float* __restrict__ sT, cons
 // slots of a 16-trajectory group and its 8 channels of o' (the stages lh_score / lh_exp / lh_norm / lh_mfma of the cooperative kernel
 // in a row) -- at the start of the glimpse phase on the waves that finish that phase first, the tail on one wave per group in the
 // pointer phase (out of line: their ~250 live registers must not shape the register allocation of the streaming loops).
-static __device__ __attribute__((noinline)) void co_local_head_call(const float* sT, const float* sXrows, float* sO1, int h, int lo, int hi) {
+// Their pointers keep the LDS address space across the call: 32 bits each, plain LDS instructions inside.
+typedef __attribute__((address_space(3))) float lds_float;
+__device__ __forceinline__ lds_float* as_lds(float* p) { return (lds_float*)p; }
+static __device__ __attribute__((noinline)) void co_local_head_call(const lds_float* sT_, const lds_float* sXrows_, lds_float* sO1_, int h, int lo, int hi) {
+    const float *sT = (const float*)sT_, *sXrows = (const float*)sXrows_;
+    float* sO1 = (float*)sO1_;
     const float* LX = sXrows + lo * CO_XP;
     const int dt = h >> 1;
     f32x4c lf[3][3], lal[3];
@@ -246,8 +251,9 @@ static __device__ __attribute__((noinline)) void co_local_head_call(const float*
         *reinterpret_cast<float4*>(sO1 + (dt * 64 + 16 * hi + lo) * 4) = make_float4(xo[0], xo[1], xo[2], xo[3]);
     }
 }
-static __device__ __attribute__((noinline)) void co_local_tail_call(const float* sT, float* sXrows, const float* sO1, int lo, int hi) {
-    co_local_tail(sT, sXrows, sO1, sXrows + CO_XU, CO_XP, lo, hi);
+static __device__ __attribute__((noinline)) void co_local_tail_call(const lds_float* sT_, lds_float* sXrows_, const lds_float* sO1, int lo, int hi) {
+    float* sXrows = (float*)sXrows_;
+    co_local_tail((const float*)sT_, sXrows, (const float*)sO1, sXrows + CO_XU, CO_XP, lo, hi);
 }
 
 template <bool TSP>

@@ -1103,7 +1103,7 @@ __global__ __launch_bounds__(512) void rollout_fwd_mt_kernel(const elg_rollout_a
                 // local policy, stage 1: head unit (group w >> 2, head w & 3) on wave w; o' waits in the per-wave scratch area
                 // (free between the owners' phases) for the tail in the pointer phase
                 if (A.has_local && wave < 4 * NG)
-                    co_local_head_call(sT, sX + (wave >> 2) * 16 * CO_XP, sdem + ((N1 + 3) & ~3) + (wave >> 2) * 512, wave & 3, lo, hi);
+                    co_local_head_call(as_lds(sT), as_lds(sX + (wave >> 2) * 16 * CO_XP), as_lds(sdem + ((N1 + 3) & ~3) + (wave >> 2) * 512), wave & 3, lo, hi);
                 if constexpr (BF) {
                     // ---- bf16 mode: one instruction per score tile, one per PAIR of node tiles for the output
                     u32x4 qb1[NG];
@@ -1272,7 +1272,7 @@ __global__ __launch_bounds__(512) void rollout_fwd_mt_kernel(const elg_rollout_a
             // ================= pointer: node tiles over the waves; local-policy tail of group g: wave 7 - g =================
             // (the tail costs about what one node tile does: its wave joins the tile round-robin one round late)
             const int nloc = A.has_local ? NG : 0, W0 = 8 - nloc, skip = nloc ? W0 : 0;
-            if (wave >= W0) co_local_tail_call(sT, sX + (7 - wave) * 16 * CO_XP, sdem + ((N1 + 3) & ~3) + (7 - wave) * 512, lo, hi);
+            if (wave >= W0) co_local_tail_call(as_lds(sT), as_lds(sX + (7 - wave) * 16 * CO_XP), as_lds(sdem + ((N1 + 3) & ~3) + (7 - wave) * 512), lo, hi);
             {
                 // s^T[node][trajectory] = sum over the channels of PK[node][c] o[trajectory][c] on v_mfma_f32_16x16x32_bf16:
                 // per 32 channels the six term products a1 b1, a1 b2, a2 b1, a2 b2, a1 b3, a3 b1 (24 instructions of 16 cycles per
@@ -2164,7 +2164,7 @@ __global__ __launch_bounds__(512) void rollout_fwd_xm_kernel(const elg_rollout_a
                 f32x4c o = {0.f, 0.f, 0.f, 0.f}, o2 = {0.f, 0.f, 0.f, 0.f};
                 __syncthreads();        // every head has its queries: the rows are free for the term planes of o
                 // local policy, stage 1: the four head units on the waves that finish the glimpse first (as in the streaming kernel)
-                if (A.has_local && wave < 4) co_local_head_call(sT, sX, sdem + ((N1 + 3) & ~3), wave & 3, lo, hi);
+                if (A.has_local && wave < 4) co_local_head_call(as_lds(sT), as_lds(sX), as_lds(sdem + ((N1 + 3) & ~3)), wave & 3, lo, hi);
                 auto softmax_update = [&](f32x4c (&S)[TU]) {
                     float tm = ELG_NEG_INF;
 #pragma unroll
@@ -2275,7 +2275,7 @@ __global__ __launch_bounds__(512) void rollout_fwd_xm_kernel(const elg_rollout_a
             __syncthreads();
             // ================= pointer: node tiles over the waves; the local policy's tail on wave 7 =================
             const int nloc = A.has_local ? 1 : 0, W0 = 8 - nloc, skip = nloc ? W0 : 0;
-            if (wave >= W0) co_local_tail_call(sT, sX, sdem + ((N1 + 3) & ~3), lo, hi);
+            if (wave >= W0) co_local_tail_call(as_lds(sT), as_lds(sX), as_lds(sdem + ((N1 + 3) & ~3)), lo, hi);
             {
                 int nt = (wave < W0 ? wave : skip + wave);
                 float* orow = rows + (size_t)lo * NP + 4 * hi;

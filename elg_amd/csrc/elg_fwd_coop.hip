@@ -1185,7 +1185,7 @@ __global__ __launch_bounds__(1024) void rollout_fwd_coop3_kernel(const elg_rollo
                     if (TRAIN && live && !(ELG_EXP_SKIP & 4)) *reinterpret_cast<float4*>(A.trO + ((size_t)b * Rcap + r) * ELG_E + 16 * wg + 4 * hi_t) = ov;
                 }
                 // local policy, stage 1: the group's four head units on waves 4-7 (which carry no trajectories), after their glimpse unit
-                if ((LEAN || A.has_local) && wg >= 4) co_local_head_call(sT, sX + grp * 16 * CO_XP, sO1 + grp * 512, wg - 4, lo_t, hi_t);
+                if ((LEAN || A.has_local) && wg >= 4) co_local_head_call(as_lds(sT), as_lds(sX + grp * 16 * CO_XP), as_lds(sO1 + grp * 512), wg - 4, lo_t, hi_t);
                 ELG_STAMP(sc, 0);
                 grp8_barrier(gcnt, bar_target, lane);
                 ELG_STAMP(sc, 1);
@@ -1227,7 +1227,7 @@ __global__ __launch_bounds__(1024) void rollout_fwd_coop3_kernel(const elg_rollo
                             make_float4(a0[0] + a1[0], a0[1] + a1[1], a0[2] + a1[2], a0[3] + a1[3]);
                     }
                 } else if (LEAN || A.has_local) {
-                    co_local_tail_call(sT, sX + grp * 16 * CO_XP, sO1 + grp * 512, lo_t, hi_t);
+                    co_local_tail_call(as_lds(sT), as_lds(sX + grp * 16 * CO_XP), as_lds(sO1 + grp * 512), lo_t, hi_t);
                 }
                 ELG_STAMP(sc, 2);
                 grp8_barrier(gcnt, bar_target, lane);
