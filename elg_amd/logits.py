@@ -238,7 +238,7 @@ def verify_draft(target_probs: torch.Tensor, draft_tokens: torch.Tensor, uniform
     """Which drafted choices the target keeps, and what it answers instead of the first one it does not: speculative sampling from given
     uniforms.  target_probs (..., G + 1, V): the target's probabilities at each draft and after the last; draft_tokens (..., G) int32 /
     int64; uniforms (..., G + 1) f32 in [0, 1): one per acceptance test and, last, one for the draw; draft_probs (..., G, V) of the same
-    type, or None where the drafts were certain (greedy); lengths (...) int32: drafts of each sequence (clamped to 0 .. G), None: all G.
+    type, or None where the drafts were certain (greedy); lengths (...) int32 / int64: drafts of each sequence (clamped to 0 .. G), None: all G.
 
     Returns tokens (..., G + 1) int32 -- the accepted drafts, the drawn choice, then -1 -- and accepted (...) int32.  A draft is kept while
     u q(x) < p(x) (exact, in 64 bits); the draw is from max(p - q, 0) at the refused draft, from the target's next row if none was refused,
@@ -273,7 +273,9 @@ def verify_draft(target_probs: torch.Tensor, draft_tokens: torch.Tensor, uniform
         _beside(lengths, dev, "lengths")
         if lengths.shape != lead or lengths.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"lengths must be {tuple(lead)} int32 or int64, got {tuple(lengths.shape)} {lengths.dtype}")
-        lengths = lengths.to(torch.int32).contiguous()
+        if lengths.dtype is torch.int64:
+            lengths = lengths.clamp(0, G).to(torch.int32)       # clamped before it is cut to 32 bits
+        lengths = lengths.contiguous()
     tokens = p.new_empty((*lead, G + 1), dtype=torch.int32)
     accepted = p.new_empty(lead, dtype=torch.int32)
     lib, ws, n = L.lib(), None, 0

@@ -416,6 +416,14 @@ def test_verify_sizes(V, dtype):
     check_verify(p, x.long(), u, None, n.long())
 
 
+def test_verify_lengths_beyond_32_bits_are_clamped():
+    p, q, x, u = drafts(6, 3, 40, 5)
+    n = torch.tensor([2 ** 32, 2 ** 32 + 1, -2 ** 32, 2 ** 40, 3, 2 ** 31])
+    got = lg().verify_draft(p.to(DEV), x.to(DEV), u.to(DEV), draft_probs=q.to(DEV), lengths=n.to(DEV))
+    want = lg().verify_draft(p.to(DEV), x.to(DEV), u.to(DEV), draft_probs=q.to(DEV), lengths=n.clamp(0, 3).int().to(DEV))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_verify_borders_are_exact():
     p = torch.tensor([[[0.25, 0.25, 0.5], [0.5, 0.0, 0.5]]]).repeat(7, 1, 1)
     q = torch.tensor([[[0.5, 0.25, 0.25]]]).repeat(7, 1, 1)
