@@ -253,6 +253,9 @@ __device__ __noinline__ void top_row_again(const TopArgs& A, long long r, TopSha
     int found = sh.n_cand, tie_need = 0;
     unsigned tie_key = 0;
     if (found > TOP_CAP) {
+        // every wave has its count before n_cand starts over: where the bound is the NaN key already the search below takes no step, and none of
+        // its barriers stands between
+        __syncthreads();
         // the k-th largest key of all elements: count(>= lo) >= k holds throughout
         hi = 0xFFFFFFFFu;
         while (lo < hi) {
