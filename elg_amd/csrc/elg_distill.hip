@@ -629,7 +629,11 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistillArgs A)
             const float d = gsum<G>(sd);
             float L = 0.f;
             if (!(a >= 1.f)) L = (d * q_scale) * A.c2 + (1.f - a) * lg2(q_scale * S);
-            if (a > TINY_MASS) L += a * (lg2(a * S * inv_sr) - (m_rest - m) * A.c2);
+            if (a > TINY_MASS) {
+                // v_log_f32 takes a subnormal for 0, and a S / sr can be one long before a is: a small mass goes in 2^64 times as large
+                const bool small = a < 1e-18f;
+                L += a * (lg2((small ? a * 0x1p64f : a) * S * inv_sr) - (small ? 64.f : 0.f) - (m_rest - m) * A.c2);
+            }
             L = live ? L * (LN2 * A.tau * A.tau * x.w) : 0.f;
             if (l == 0 && valid) {
                 if (A.loss_rows) A.loss_rows[r] = L * A.scale;

@@ -45,3 +45,38 @@ def test_top_of_rows_with_thousands_of_nan(V, k, dtype):
         np.testing.assert_array_equal(idx.cpu().numpy(), ri)
         np.testing.assert_array_equal(host(values), rv)
         assert torch.isnan(tail[:10]).all() and torch.isfinite(tail[10:]).all()
+
+
+# ----------------------------------------------------------------------------------------------------------- distillation
+def check_losses(z, tv, ti, a, tau=1.0, w=None, R=None):
+    """Losses of the rows and their mean against the definition, within its bounds; the gradient too."""
+    d = [None if t is None else t.to(DEV) for t in (z, tv, ti, a, w)]
+    loss, grad = lg().distill_loss_grad(d[0], d[1], d[2], tail=d[3], temperature=tau, weight=d[4], reduction="none")
+    rl, rg, lb, gb = ro.distill(host(z), host(tv), ti.numpy(), host(a), tau, None if w is None else host(w))
+    got, fin = host(loss), np.isfinite(rl)
+    assert (got[~fin] == rl[~fin]).all(), (got, rl)
+    assert (np.abs(got[fin] - rl[fin]) <= lb[fin] + 1e-30).all(), (got, rl, lb)
+    assert (np.abs(host(grad) - rg) <= gb + 4 * ro.U * np.abs(rg) + ro.TINY["float32"]).all()
+    mean = lg().distill_loss(d[0], d[1], d[2], tail=d[3], temperature=tau, weight=d[4]).item()
+    if fin.all():
+        assert abs(mean - rl.mean()) <= lb.mean() + 2 * ro.U * abs(rl.mean()) + 1e-30
+    else:
+        assert mean == np.inf
+    return got, rl
+
+
+TINY_TAILS = [1e-45, 1e-40, 1.2e-38, 1e-37, 2e-36, 1e-35, 1e-33, 1e-30, 1e-25, 1e-19, 1.1e-18, 1e-10]
+
+
+@pytest.mark.parametrize("V", [17, 250, 1001, 2048, 2049, 9001])
+def test_distill_tiny_tail_over_a_flat_rest(V):
+    """The teacher leaves next to nothing outside its entries and the student has hundreds of nodes there, all alike: tail S / p_rest lies below
+    the smallest normal number, and its logarithm is still finite."""
+    k, n = 5, len(TINY_TAILS)
+    z = torch.full((n, V), -50.0)
+    z[:, 0] = 50.0
+    z[1::2, 0] = -49.0                                     # the best node inside the rest's reach as well
+    tv, ti = torch.tensor([40.0, -48.0, -49.0, -49.5, -50.0]).expand(n, k).contiguous(), torch.arange(k).int().expand(n, k).contiguous()
+    a = torch.tensor(TINY_TAILS, dtype=torch.float64).float()
+    got, _ = check_losses(z, tv, ti, a)
+    assert np.isfinite(got).all()
