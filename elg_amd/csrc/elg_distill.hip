@@ -37,7 +37,6 @@ struct DistillArgs {
     long long g_stride;                   // bytes
 };
 
-constexpr float TINY_MASS = 1e-36f;       // a (log a - log p_rest) below this is nothing in f32
 // the loss is formed in base 2, like the exponentials, and brought to base e at its end
 constexpr float LN2 = 0.6931471805599453f;
 __device__ __forceinline__ float lg2(float x) { return __builtin_amdgcn_logf(x); }       // v_log_f32
@@ -629,10 +628,11 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistillArgs A)
             const float d = gsum<G>(sd);
             float L = 0.f;
             if (!(a >= 1.f)) L = (d * q_scale) * A.c2 + (1.f - a) * lg2(q_scale * S);
-            if (a > TINY_MASS) {
+            if (a > 0.f) {
                 // v_log_f32 takes a subnormal for 0, and a S / sr can be one long before a is: a small mass goes in 2^64 times as large
                 const bool small = a < 1e-18f;
-                L += a * (lg2((small ? a * 0x1p64f : a) * S * inv_sr) - (small ? 64.f : 0.f) - (m_rest - m) * A.c2);
+                const float d_rest = lg2((small ? a * 0x1p64f : a) * S * inv_sr) - (small ? 64.f : 0.f) - (m_rest - m) * A.c2;
+                L += sr <= 0.f ? -ELG_NEG_INF : a * d_rest;        // any mass on a rest that the student has closed
             }
             L = live ? L * (LN2 * A.tau * A.tau * x.w) : 0.f;
             if (l == 0 && valid) {

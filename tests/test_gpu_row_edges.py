@@ -80,3 +80,24 @@ def test_distill_tiny_tail_over_a_flat_rest(V):
     a = torch.tensor(TINY_TAILS, dtype=torch.float64).float()
     got, _ = check_losses(z, tv, ti, a)
     assert np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("V", [16, 17, 250, 257, 1001, 2048, 2049, 9001, 70001])
+def test_distill_any_tail_over_a_closed_rest_is_infinite(V):
+    """The student has closed every node that is no entry's, or the entries are all of its open nodes: any mass of the teacher there, however
+    small, makes the loss +inf, in rows of every length; no mass makes none."""
+    k = 9
+    a = torch.tensor(TINY_TAILS + [0.25, 0.0], dtype=torch.float64).float()
+    z = torch.full((len(a), V), -np.inf)
+    z[:, :k] = torch.linspace(-3, 3, k)
+    tv, ti = torch.zeros(len(a), k), torch.arange(k).int().expand(len(a), k).contiguous()
+    got, _ = check_losses(z, tv, ti, a)
+    assert (got[:-1] == np.inf).all() and np.isfinite(got[-1])
+
+
+@pytest.mark.parametrize("k", [9, 20, 100, 200])
+def test_distill_any_tail_where_the_entries_are_all_nodes(k):
+    a = torch.tensor(TINY_TAILS + [0.25, 0.0], dtype=torch.float64).float()
+    z = torch.linspace(-3, 3, k).expand(len(a), k).contiguous()
+    got, _ = check_losses(z, torch.zeros(len(a), k), torch.arange(k).int().expand(len(a), k).contiguous(), a)
+    assert (got[:-1] == np.inf).all() and np.isfinite(got[-1])
