@@ -551,7 +551,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistillArgs A)
         float q[KE], st = 0.f, sz = 0.f;
 #pragma unroll
         for (int e = 0; e < KE; ++e) {
-            q[e] = at[e] >= 0 ? ex2((x.t[e] - tm) * A.c2) : 0.f;
+            q[e] = at[e] >= 0 ? fabsf(ex2((x.t[e] - tm) * A.c2)) : 0.f;       // (a NaN can carry a sign: only the mark is to have one)
             st += q[e];
         }
         auto clear = [&]() {
@@ -652,14 +652,26 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistillArgs A)
                     x.z[n] = live ? x.z[n] : 0.f;
                     qv[n] = live ? qv[n] : 0.f;
                 }
-            if (valid) {
-                elem_t<DT>* grow = reinterpret_cast<elem_t<DT>*>(A.grad + r * A.g_stride) + l;
+            elem_t<DT>* grow = reinterpret_cast<elem_t<DT>*>(A.grad + r * A.g_stride) + l;
+            auto put = [&](int n, float gn) {
+                if (n * G + G <= V) grow[n * G] = (elem_t<DT>)gn;
+                else if (l < V - n * G) grow[n * G] = (elem_t<DT>)gn;
+            };
+            // A NaN or infinity among the teacher's logits or in the cotangent: the masses stay with the entries' nodes, and the difference is
+            // formed before it is scaled (infinity less infinity).  In other rows a node of no entry adds Gq (-0), which changes nothing.
+            const bool odd = live && !(fabsf(Gq) < -ELG_NEG_INF);
+            if (__any(odd)) {
+                const float p_top = f_top * inv_S;
+                if (valid)
 #pragma unroll
-                for (int n = 0; n < NE; ++n) {
-                    const float gn = fmaf(x.z[n], f2i(qv[n]) < 0 ? c_rest : c_top, -Gq * qv[n]);
-                    if (n * G + G <= V) grow[n * G] = (elem_t<DT>)gn;
-                    else if (l < V - n * G) grow[n * G] = (elem_t<DT>)gn;
-                }
+                    for (int n = 0; n < NE; ++n) {
+                        const bool rest = f2i(qv[n]) < 0;
+                        const float usual = fmaf(x.z[n], rest ? c_rest : c_top, -Gq * qv[n]);
+                        put(n, odd ? rest ? x.z[n] * c_rest : Gr * (x.z[n] * p_top - qv[n] * q_scale) : usual);
+                    }
+            } else if (valid) {
+#pragma unroll
+                for (int n = 0; n < NE; ++n) put(n, fmaf(x.z[n], f2i(qv[n]) < 0 ? c_rest : c_top, -Gq * qv[n]));
             }
         }
         if (!AHEAD) next.load(A, r + step, w_next, l, plain_entries);

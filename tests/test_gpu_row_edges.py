@@ -101,3 +101,31 @@ def test_distill_any_tail_where_the_entries_are_all_nodes(k):
     z = torch.linspace(-3, 3, k).expand(len(a), k).contiguous()
     got, _ = check_losses(z, torch.zeros(len(a), k), torch.arange(k).int().expand(len(a), k).contiguous(), a)
     assert (got[:-1] == np.inf).all() and np.isfinite(got[-1])
+
+
+@pytest.mark.parametrize("V", [33, 101, 250, 1001, 2048, 2049, 9001, 70001])
+def test_distill_non_finite_teachers_and_cotangents_reach_what_the_formula_says(V):
+    """A NaN or +inf among the teacher's entries is in every q of its row and in no p: the entries' nodes get NaN, the others keep their gradient.
+    An infinite cotangent makes infinite gradients of the formula's signs.  The same in rows of every length."""
+    R, k = 6, 7
+    g = rng(V)
+    z = torch.randn(R, V, generator=g) * 2
+    tv, ti = torch.randn(R, k, generator=g), torch.stack([torch.randperm(V, generator=g)[:k] for _ in range(R)]).int()
+    a = torch.full((R,), 0.2)
+    good = lg().distill_loss_grad(z.to(DEV), tv.to(DEV), ti.to(DEV), tail=a.to(DEV), reduction="none")
+    bad = tv.clone()
+    bad[1, 3], bad[4, 0] = float("nan"), float("inf")
+    loss, grad = lg().distill_loss_grad(z.to(DEV), bad.to(DEV), ti.to(DEV), tail=a.to(DEV), reduction="none")
+    entry = torch.zeros(R, V, dtype=torch.bool, device=DEV).scatter_(1, ti.long().to(DEV), True)
+    odd = torch.zeros(R, 1, dtype=torch.bool, device=DEV)
+    odd[[1, 4]] = True
+    assert torch.equal(torch.isnan(grad), entry & odd) and torch.equal(grad[~(entry & odd)], good[1][~(entry & odd)])
+    assert torch.isnan(loss[[1, 4]]).all() and torch.equal(loss[[0, 2, 3, 5]], good[0][[0, 2, 3, 5]])
+    # the cotangent, with a row that has no gradient among them
+    z[2] = -np.inf
+    x = z.to(DEV).requires_grad_(True)
+    cot = torch.tensor([1.0, np.inf, np.inf, -np.inf, 1.0, float("nan")], device=DEV)
+    (gx,) = torch.autograd.grad(lg().distill_loss(x, tv.to(DEV), ti.to(DEV), tail=a.to(DEV), reduction="none"), x, cot)
+    assert torch.equal(gx[[0, 4]], good[1][[0, 4]]) and (gx[2] == 0).all() and torch.isnan(gx[5]).all()
+    for r, sign in ((1, 1.0), (3, -1.0)):
+        assert torch.equal(gx[r], torch.sign(good[1][r]) * sign * np.inf)
