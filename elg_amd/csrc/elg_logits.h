@@ -12,6 +12,9 @@ namespace elg {
 int fail(int code, const std::string& msg);
 int launch_status(const char* what);
 
+// Workgroups of 256 threads that one launch can have: its threads are counted in 32 bits, and beyond them the grid wraps without an error.
+constexpr long long LAUNCH_WG = 0xFFFFFFFFLL / 256;
+
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));

@@ -346,16 +346,32 @@ int segments(int64_t V, int type) {
 }
 
 template <int DT>
-void launch(const VerifyArgs& A, int64_t B, double2* parts, hipStream_t s) {
-    const int segs = segments(A.V, DT);
+void launch_part(const VerifyArgs& A, long long B, int segs, double2* parts, hipStream_t s) {
     const dim3 waves((unsigned)((B + 3) / 4)), all((unsigned)B);
-    if (A.V <= 128) hipLaunchKernelGGL((verify_wave_kernel<DT, 2>), waves, dim3(256), 0, s, A, (long long)B);
-    else if (A.V <= 512) hipLaunchKernelGGL((verify_wave_kernel<DT, 8>), waves, dim3(256), 0, s, A, (long long)B);
-    else if (A.V <= 1024) hipLaunchKernelGGL((verify_wave_kernel<DT, 16>), waves, dim3(256), 0, s, A, (long long)B);
+    if (A.V <= 128) hipLaunchKernelGGL((verify_wave_kernel<DT, 2>), waves, dim3(256), 0, s, A, B);
+    else if (A.V <= 512) hipLaunchKernelGGL((verify_wave_kernel<DT, 8>), waves, dim3(256), 0, s, A, B);
+    else if (A.V <= 1024) hipLaunchKernelGGL((verify_wave_kernel<DT, 16>), waves, dim3(256), 0, s, A, B);
     else if (segs == 1) hipLaunchKernelGGL((verify_row_kernel<DT>), all, dim3(256), 0, s, A);
     else {
         hipLaunchKernelGGL((verify_part_kernel<DT>), dim3((unsigned)(B * segs)), dim3(256), 0, s, A, parts, segs);
         hipLaunchKernelGGL((verify_pick_kernel<DT>), all, dim3(256), 0, s, A, (const double2*)parts, segs);
+    }
+}
+// as many sequences at a time as a launch has workgroups for
+template <int DT>
+void launch(const VerifyArgs& A, long long B, double2* parts, hipStream_t s) {
+    const int segs = segments(A.V, DT);
+    const long long at_once = A.V <= 1024 ? 4 * LAUNCH_WG : LAUNCH_WG / segs;
+    for (long long b = 0; b < B; b += at_once) {
+        VerifyArgs C = A;
+        C.p += b * A.pb;
+        if (A.q) C.q += b * A.qb;
+        C.tok = (const char*)A.tok + b * A.tok_stride * (A.tok_wide ? 8 : 4);
+        C.u += b * A.u_stride;
+        if (A.lengths) C.lengths += b;
+        C.out += b * (A.G + 1);
+        C.accepted += b;
+        launch_part<DT>(C, B - b < at_once ? B - b : at_once, segs, parts, s);         // (parts: read before the next ones are written)
     }
 }
 
@@ -383,7 +399,6 @@ extern "C" int elg_verify_draft(const void* target, int64_t target_bstride, int6
     if (((uintptr_t)target | (uintptr_t)draft) % es || (uintptr_t)tokens % (tokens_wide ? 8 : 4)) return fail(ELG_EINVAL, "verify_draft: misaligned buffer");
     const int64_t need = elg_verify_ws_bytes(B, V, type);
     if (need > 0 && (!ws || ws_bytes < need || (uintptr_t)ws % 16)) return fail(ELG_EINVAL, "verify_draft: needs elg_verify_ws_bytes() of scratch");
-    if (need / 16 > 0x7FFFFFFF) return fail(ELG_EINVAL, "verify_draft: too many long rows for one call");
     VerifyArgs A;
     A.p = (const char*)target; A.q = (const char*)draft;
     A.pb = target_bstride * es; A.ps = target_sstride * es; A.qb = draft_bstride * es; A.qs = draft_sstride * es;

@@ -129,3 +129,40 @@ def test_distill_non_finite_teachers_and_cotangents_reach_what_the_formula_says(
     assert torch.equal(gx[[0, 4]], good[1][[0, 4]]) and (gx[2] == 0).all() and torch.isnan(gx[5]).all()
     for r, sign in ((1, 1.0), (3, -1.0)):
         assert torch.equal(gx[r], torch.sign(good[1][r]) * sign * np.inf)
+
+
+# ----------------------------------------------------------------------------------------------------------- verification
+def test_verify_of_more_sequences_than_one_launch_takes():
+    """2^26 and a few short sequences, one wave each: over 2^32 threads."""
+    B, V = 2 ** 26 + 5, 2
+    g = torch.Generator(device=DEV).manual_seed(1)
+    p = torch.rand(B, 2, V, device=DEV, generator=g, dtype=torch.bfloat16)
+    u = torch.rand(B, 2, device=DEV, generator=g)
+    x = torch.randint(0, V, (B, 1), device=DEV, generator=g, dtype=torch.int32)
+    tok, acc = lg().verify_draft(p, x, u)
+    kept = u[:, 0].double() < p[:, 0].gather(1, x.long())[:, 0].double()
+    assert torch.equal(acc, kept.int())
+    row = torch.where(kept[:, None], p[:, 1], p[:, 0])
+    left = row.masked_fill(~kept[:, None] & (torch.arange(V, device=DEV) == x), 0.0)
+    row = torch.where((left.sum(1) > 0)[:, None], left, row).double()
+    drawn = torch.where(row[:, 0] > u[:, 1].double() * row.sum(1), 0, 1).int()
+    drawn[row.sum(1) == 0] = -1
+    assert torch.equal(tok[:, 0], torch.where(kept, x[:, 0], drawn)) and torch.equal(tok[:, 1], torch.where(kept, drawn, -1))
+
+
+@pytest.mark.parametrize("B,V", [(2 ** 24 + 8, 1100), (5_600_000, 8300)])
+def test_verify_of_more_long_rows_than_one_launch_takes(B, V):
+    """One target and one draft over and over as expanded views, a workgroup or three to a sequence."""
+    n, G = 1000, 2
+    g = rng(V)
+    p, q = torch.softmax(torch.randn(1, G + 1, V, generator=g) * 3, -1), torch.softmax(torch.randn(1, G, V, generator=g) * 3, -1)
+    x, u = torch.multinomial(q[0], n, replacement=True, generator=g).T.contiguous().int(), torch.rand(n, G + 1, generator=g)
+    lengths = torch.randint(0, G + 1, (n,), generator=g).int()
+    rt, ra = ro.verify(host(p.expand(n, G + 1, V))[:50], x[:50].numpy(), host(u)[:50], host(q.expand(n, G, V))[:50], lengths[:50].numpy())
+    P, Q = p.to(DEV), q.to(DEV)
+    few = lg().verify_draft(P.expand(n, G + 1, V), x.to(DEV), u.to(DEV), draft_probs=Q.expand(n, G, V), lengths=lengths.to(DEV))
+    np.testing.assert_array_equal(few[0][:50].cpu().numpy(), rt)
+    np.testing.assert_array_equal(few[1][:50].cpu().numpy(), ra)
+    tile = lambda t: t.repeat(-(-B // n), *[1] * (t.dim() - 1))[:B].to(DEV)  # noqa: E731
+    many = lg().verify_draft(P.expand(B, G + 1, V), tile(x), tile(u), draft_probs=Q.expand(B, G, V), lengths=tile(lengths))
+    assert torch.equal(many[0], tile(few[0])) and torch.equal(many[1], tile(few[1]))
