@@ -35,6 +35,19 @@ struct DistillArgs {
     float4* rec;                          // two a row: what a long row's loss is formed from; or null
     char* grad;                           // (R, V) packed, or null
     long long g_stride;                   // bytes
+    // the rows from r on, for a kernel that leaves its losses in rec
+    DistillArgs from(long long r) const {
+        DistillArgs C = *this;
+        C.z += r * z_stride;
+        C.tv = (const char*)tv + r * k * (tv_type == ELG_F32 ? 4 : 2);
+        C.ti = (const char*)ti + r * k * (ti_wide ? 8 : 4);
+        if (tail) C.tail += r;
+        if (weight) C.weight += r;
+        if (cot) C.cot += r * cot_stride;
+        if (rec) C.rec += 2 * r;
+        if (grad) C.grad += r * g_stride;
+        return C;
+    }
 };
 
 // the loss is formed in base 2, like the exponentials, and brought to base e at its end
@@ -759,8 +772,13 @@ void launch(const DistillArgs& A, const Plan& P, float2* parts, hipStream_t s) {
         else fits(64, 8) ? launch_small<DT, 64, 8, 4>(A, grid, s) : fits(64, 16) ? launch_small<DT, 64, 16, 4>(A, grid, s) : launch_small<DT, 64, 32, 4>(A, grid, s);
     } else if (P.split) {
         const int grad_segs = A.grad ? P.segs : 1;
-        hipLaunchKernelGGL((distill_part_kernel<DT>), dim3((unsigned)(A.R * P.segs)), dim3(SEG_T), 0, s, A, parts, P.segs);
-        hipLaunchKernelGGL((distill_join_kernel<DT>), dim3((unsigned)(A.R * grad_segs)), dim3(SEG_T), 0, s, A, parts, P.segs, grad_segs);
+        const long long at_once = LAUNCH_WG / P.segs;          // rows of a launch
+        for (long long r = 0; r < A.R; r += at_once) {
+            const long long n = A.R - r < at_once ? A.R - r : at_once;
+            const DistillArgs C = A.from(r);
+            hipLaunchKernelGGL((distill_part_kernel<DT>), dim3((unsigned)(n * P.segs)), dim3(SEG_T), 0, s, C, parts, P.segs);
+            hipLaunchKernelGGL((distill_join_kernel<DT>), dim3((unsigned)(n * grad_segs)), dim3(SEG_T), 0, s, C, parts, P.segs, grad_segs);
+        }
     } else if (nch <= 256 * 4) launch_row<DT, 256, 4>(A, grid, s);
     else if (nch <= 256 * 8) launch_row<DT, 256, 8>(A, grid, s);
     else if (nch <= 256 * 16) launch_row<DT, 256, 16>(A, grid, s);
@@ -794,7 +812,6 @@ extern "C" int elg_distill_loss_grad(const void* z, int64_t z_stride, int type, 
     const Plan P(R, V, type);
     const bool want_loss = loss_rows || loss_total, scratch = P.split || (P.lanes ? loss_total && P.parts > 1 : want_loss);
     if (R > 0 && scratch && (!ws || ws_bytes < P.bytes(R))) return fail(ELG_EINVAL, "distill: needs elg_distill_ws_bytes() of scratch");
-    if (P.split && R * P.segs > 0x7FFFFFFF) return fail(ELG_EINVAL, "distill: too many long rows for one call");
     if (R == 0 && !loss_total) return ELG_OK;
     const int es = type == ELG_F32 ? 4 : 2;
     if (((uintptr_t)z | (uintptr_t)grad) % es || (uintptr_t)top_values % (top_type == ELG_F32 ? 4 : 2) || (uintptr_t)top_idx % (idx_wide ? 8 : 4) || (uintptr_t)ws % 16)

@@ -131,6 +131,23 @@ def test_distill_non_finite_teachers_and_cotangents_reach_what_the_formula_says(
         assert torch.equal(gx[r], torch.sign(good[1][r]) * sign * np.inf)
 
 
+def test_distill_of_more_segments_than_one_launch_takes():
+    """One row over and over as an expanded view: 990 000 rows of 17 segments are over 2^32 threads."""
+    V, R, n = 65600, 990_000, 1000
+    g = rng(3)
+    z = torch.randn(1, V, generator=g)
+    tv, ti, a, w = torch.randn(n, 2, generator=g), torch.randint(0, V, (n, 2), generator=g).int(), torch.rand(n, generator=g), torch.rand(n, generator=g)
+    few = lg().distill_loss(z.expand(n, V).to(DEV), tv.to(DEV), ti.to(DEV), tail=a.to(DEV), weight=w.to(DEV), reduction="none")
+    rl, _, lb, _ = ro.distill(host(z.expand(20, V)), host(tv[:20]), ti[:20].numpy(), host(a[:20]), 1.0, host(w[:20]))
+    assert (np.abs(host(few)[:20] - rl) <= lb + 1e-30).all()
+    tile = lambda t: t.repeat(R // n, *[1] * (t.dim() - 1)).to(DEV)  # noqa: E731
+    more = dict(tail=tile(a), weight=tile(w))
+    many = lg().distill_loss(z.to(DEV).expand(R, V), tile(tv), tile(ti), reduction="none", **more)
+    assert torch.equal(many.view(-1, n), few.expand(R // n, n))
+    total = lg().distill_loss(z.to(DEV).expand(R, V), tile(tv), tile(ti), reduction="sum", **more)
+    assert total.item() == pytest.approx(many.double().sum().item(), rel=1e-6)
+
+
 # ----------------------------------------------------------------------------------------------------------- verification
 def test_verify_of_more_sequences_than_one_launch_takes():
     """2^26 and a few short sequences, one wave each: over 2^32 threads."""
