@@ -112,17 +112,15 @@ class _Teacher:
         dev = logits.get_device()
         _beside(values, dev, "top_values")
         _beside(idx, dev, "top_idx")
-        self.top_type = _TYPES.get(values.dtype)
-        if self.top_type is None:
+        if values.dtype not in _TYPES:
             raise ValueError(f"top_values must be float32, bfloat16 or float16, got {values.dtype}")
         if idx.dtype is not torch.int32 and idx.dtype is not torch.int64:
             raise ValueError(f"top_idx must be int32 or int64, got {idx.dtype}")
         lead = logits.shape[:-1]
         if values.shape != idx.shape or values.dim() == 0 or values.shape[:-1] != lead:
             raise ValueError(f"top_values and top_idx must be {tuple(lead)} + (k,), got {tuple(values.shape)} and {tuple(idx.shape)}")
-        self.k = values.shape[-1]
-        if not 1 <= self.k <= L.TOP_MAX_K:
-            raise ValueError(f"1 .. {L.TOP_MAX_K} teacher entries a row, got {self.k}")
+        if not 1 <= values.shape[-1] <= L.TOP_MAX_K:
+            raise ValueError(f"1 .. {L.TOP_MAX_K} teacher entries a row, got {values.shape[-1]}")
         if (values.requires_grad or (tail is not None and tail.requires_grad) or (weight is not None and weight.requires_grad)) \
                 and torch.is_grad_enabled():
             raise ValueError("no gradient flows to the teacher's logits, the tail or the weights: detach them")
@@ -132,17 +130,21 @@ class _Teacher:
         self.temperature = _temperature(temperature)
         self.lead = lead
 
-    def call(self, z, *, cot=None, cot_stride=0, scale=1.0, rows=None, total=None, grad=None):
-        R, V = z.shape
-        ws, n = None, 0
-        lib = L.lib()
-        if total is not None or V > 2048:
-            n = _distill_ws_bytes(R, V, self.type)
-            ws = z.new_empty(n, dtype=torch.uint8) if n else None
-        L.check(lib.elg_distill_loss_grad(_p(z), z.stride(0), self.type, R, V, _p(self.values), self.top_type, _p(self.idx),
-                                          int(self.idx.dtype == torch.int64), self.k, _p(self.tail), self.temperature, _p(self.weight),
-                                          _p(cot), cot_stride, scale, _p(rows), _p(total), _p(grad), _p(ws), n, _stream()),
-                "elg_distill_loss_grad")
+    def tensors(self):
+        return self.values, self.idx, self.tail, self.weight
+
+
+def _distill_call(z, ty, teacher, temperature, *, cot=None, cot_stride=0, scale=1.0, rows=None, total=None, grad=None):
+    values, idx, tail, weight = teacher
+    R, V = z.shape
+    ws, n = None, 0
+    lib = L.lib()
+    if total is not None or V > 2048:
+        n = _distill_ws_bytes(R, V, ty)
+        ws = z.new_empty(n, dtype=torch.uint8) if n else None
+    L.check(lib.elg_distill_loss_grad(_p(z), z.stride(0), ty, R, V, _p(values), _TYPES[values.dtype], _p(idx), int(idx.dtype == torch.int64),
+                                      values.shape[-1], _p(tail), temperature, _p(weight), _p(cot), cot_stride, scale, _p(rows), _p(total),
+                                      _p(grad), _p(ws), n, _stream()), "elg_distill_loss_grad")
 
 
 def _scale(reduction: str, R: int) -> float:
@@ -155,30 +157,37 @@ class _DistillLoss(torch.autograd.Function):
     """Forward: the loss from one read of the logits.  Backward: the gradient from a second one, scaled by the cotangent on the device."""
 
     @staticmethod
-    def forward(ctx, logits, teacher, reduction, *saved):
+    def forward(ctx, logits, teacher, reduction, values, idx, tail, weight):
         z = _rows(logits, "logits")
         scale = _scale(reduction, z.shape[0])
-        ctx.teacher, ctx.scale, ctx.reduction = teacher, scale, reduction
-        ctx.save_for_backward(logits, *saved)        # the teacher's tensors too: writing to one before the backward is an error, not a wrong gradient
+        ctx.type, ctx.temperature, ctx.scale, ctx.reduction, ctx.shape = teacher.type, teacher.temperature, scale, reduction, values.shape
+        # the teacher's tensors too, and nothing beside: writing to one before the backward is an error, not a wrong gradient, hooks on saved
+        # tensors see what the backward reads, and it is all freed with the graph
+        ctx.save_for_backward(logits, values, idx, tail, weight)
         if reduction == "none":
             loss = z.new_empty(teacher.lead, dtype=torch.float32)
             if z.shape[0]:
-                teacher.call(z, rows=loss)
+                _distill_call(z, teacher.type, (values, idx, tail, weight), teacher.temperature, rows=loss)
         else:
             loss = z.new_empty((), dtype=torch.float32)
-            teacher.call(z, total=loss, scale=scale)
+            _distill_call(z, teacher.type, (values, idx, tail, weight), teacher.temperature, total=loss, scale=scale)
         return loss
 
     @staticmethod
     def gradient(ctx, gout):
-        logits = ctx.saved_tensors[0]
+        logits, values, idx, tail, weight = ctx.saved_tensors
+        if values.shape != ctx.shape or idx.shape != ctx.shape or (tail is not None and tail.shape != ctx.shape[:-1]) \
+                or (weight is not None and weight.shape != ctx.shape[:-1]):
+            raise RuntimeError("elg_amd: a hook on saved tensors gave back a teacher of another shape than was saved")
         z = _rows(logits, "logits")
         grad = z.new_empty(logits.shape)
         if z.shape[0]:
             if gout.dtype != torch.float32 or not gout.is_contiguous():
                 gout = gout.float().contiguous()
-            ctx.teacher.call(z, cot=gout, cot_stride=int(ctx.reduction == "none"), scale=ctx.scale, grad=grad)
-        return (grad, None, None) + (None,) * (len(ctx.saved_tensors) - 1)
+            teacher = (values.contiguous(), idx.contiguous(), None if tail is None else tail.contiguous(),
+                       None if weight is None else weight.contiguous())
+            _distill_call(z, ctx.type, teacher, ctx.temperature, cot=gout, cot_stride=int(ctx.reduction == "none"), scale=ctx.scale, grad=grad)
+        return grad, None, None, None, None, None, None
 
     @staticmethod
     def backward(ctx, gout):
@@ -204,7 +213,7 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_idx: torch.
     The gradient reaches `logits` only, in their type, and can be taken once (no double backward); statistics and sums are f32, the sum over
     the rows f64."""
     t = _Teacher(logits, top_values, top_idx, tail, temperature, weight)
-    return _DistillLoss.apply(logits, t, reduction, *(x for x in (t.values, t.idx, t.tail, t.weight) if x is not None))
+    return _DistillLoss.apply(logits, t, reduction, *t.tensors())
 
 
 def distill_loss_grad(logits: torch.Tensor, top_values: torch.Tensor, top_idx: torch.Tensor, *, tail: Optional[torch.Tensor] = None,
@@ -219,10 +228,10 @@ def distill_loss_grad(logits: torch.Tensor, top_values: torch.Tensor, top_idx: t
     if reduction == "none":
         loss = z.new_empty(t.lead, dtype=torch.float32)
         if z.shape[0]:
-            t.call(z, rows=loss, grad=grad)
+            _distill_call(z, t.type, t.tensors(), t.temperature, rows=loss, grad=grad)
     else:
         loss = z.new_empty((), dtype=torch.float32)
-        t.call(z, total=loss, grad=grad, scale=scale)
+        _distill_call(z, t.type, t.tensors(), t.temperature, total=loss, grad=grad, scale=scale)
     return loss, grad
 
 

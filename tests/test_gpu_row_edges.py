@@ -131,6 +131,49 @@ def test_distill_non_finite_teachers_and_cotangents_reach_what_the_formula_says(
         assert torch.equal(gx[r], torch.sign(good[1][r]) * sign * np.inf)
 
 
+@pytest.mark.parametrize("V", [101, 3000])
+def test_distill_backward_reads_what_hooks_on_saved_tensors_give_back(V):
+    """A hook that keeps saved tensors on the host: the backward reads the copies it gives back, and the teacher's own memory is free for as long
+    as the loss waits for its backward."""
+    import weakref
+    g = rng(V)
+    z = torch.randn(6, V, generator=g).to(DEV).requires_grad_(True)
+    tv, ti = (torch.randn(6, 9, generator=g), torch.randint(0, V, (6, 9), generator=g).int())
+    a, w = torch.rand(6, generator=g), torch.rand(6, generator=g)
+    (want,) = torch.autograd.grad(lg().distill_loss(z, tv.to(DEV), ti.to(DEV), tail=a.to(DEV), weight=w.to(DEV)), z)
+    teacher = [t.to(DEV) for t in (tv, ti, a, w)]
+    alive = [weakref.ref(t) for t in teacher]
+    seen = []
+
+    def unpack(t):
+        seen.append(tuple(t.shape))
+        return t.to(DEV)
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), unpack):
+        loss = lg().distill_loss(z, teacher[0], teacher[1], tail=teacher[2], weight=teacher[3])
+    del teacher
+    assert not any(r() is not None for r in alive)
+    (got,) = torch.autograd.grad(loss, z)
+    assert torch.equal(got, want) and sorted(seen) == sorted([(6, V), (6, 9), (6, 9), (6,), (6,)])
+    # what a hook gives back is what is read: another teacher, another gradient
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.flip(0) if t.shape == (6,) else t):
+        loss = lg().distill_loss(z, tv.to(DEV), ti.to(DEV), tail=a.to(DEV), weight=w.to(DEV))
+    (got,) = torch.autograd.grad(loss, z)
+    (want,) = torch.autograd.grad(lg().distill_loss(z, tv.to(DEV), ti.to(DEV), tail=a.flip(0).to(DEV), weight=w.flip(0).to(DEV)), z)
+    assert torch.equal(got, want)
+
+
+def test_distill_teacher_is_freed_with_the_graph():
+    import weakref
+    z, ti = torch.randn(4, 50, device=DEV, requires_grad=True), torch.zeros(4, 3, device=DEV, dtype=torch.int32)
+    tv = torch.randn(4, 3, device=DEV)
+    alive = weakref.ref(tv)
+    loss = lg().distill_loss(z, tv, ti)
+    del tv
+    loss.backward()
+    assert alive() is None and z.grad is not None
+
+
 def test_distill_of_more_segments_than_one_launch_takes():
     """One row over and over as an expanded view: 990 000 rows of 17 segments are over 2^32 threads."""
     V, R, n = 65600, 990_000, 1000
