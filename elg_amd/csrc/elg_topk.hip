@@ -583,7 +583,7 @@ __global__ __launch_bounds__(256, NE == 32 ? 3 : 4) void top_sort_kernel(const T
             top = oct_sum(top);
             rest = oct_sum(rest);
             // a row without an open node gives (-inf) - (-inf) = NaN here
-            if (l == 0 && valid) A.tail[r] = m > ELG_NEG_INF || m != m ? rest * __builtin_amdgcn_rcpf(top + rest) : 0.f;
+            if (l == 0 && valid) A.tail[r] = m > ELG_NEG_INF || m != m ? rest / (top + rest) : 0.f;
         }
         wave_lds_fence();
         if (n0 * NE < k) {
@@ -827,7 +827,7 @@ __global__ __launch_bounds__(256) void top_wave_kernel(const TopArgs A) {
             }
             top = wave_sum(top);
             rest = wave_sum(rest);
-            if (lane == 0) A.tail[r] = m > ELG_NEG_INF || m != m ? rest * __builtin_amdgcn_rcpf(top + rest) : 0.f;
+            if (lane == 0) A.tail[r] = m > ELG_NEG_INF || m != m ? rest / (top + rest) : 0.f;
         }
         wave_lds_fence();
     }

@@ -47,6 +47,18 @@ def test_top_of_rows_with_thousands_of_nan(V, k, dtype):
         assert torch.isnan(tail[:10]).all() and torch.isfinite(tail[10:]).all()
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_top_tail_of_equal_logits_is_rounded_once(dtype):
+    """V equal logits: every exponential is 1 and every sum a whole number below 2^24, so that the tail is (V - k) / V after one division, which
+    is the f32 next to it."""
+    for V in (*range(2, 257), 300, 511, 777, 1001, 1500, 2047, 2049, 3001, 9001, 70001):
+        for k in sorted({1, 2, V // 3 + 1, min(V, 256) // 2 + 1}):
+            if k > min(V, 256):
+                continue
+            tail = lg().top_logits(torch.full((3, V), 1.25, dtype=TYPES[dtype], device=DEV), k, with_tail=True)[2]
+            assert (tail.cpu().numpy() == np.float32((V - k) / V)).all(), (V, k)
+
+
 # ----------------------------------------------------------------------------------------------------------- distillation
 def check_losses(z, tv, ti, a, tau=1.0, w=None, R=None):
     """Losses of the rows and their mean against the definition, within its bounds; the gradient too."""
