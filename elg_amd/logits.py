@@ -207,8 +207,9 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_idx: torch.
 
     per row; reduction 'none' (...) f32, 'sum', or 'mean' over all rows.  tail (...) f32: the teacher's probability outside its entries
     (`top_logits(with_tail=True)`), None: the entries hold everything.  weight (...) f32: 0 leaves a row out (it is not read) -- finished
-    trajectories.  Entries whose node lies outside [0, V) (-1: padding) or whose logit is -inf are absent; a node listed twice carries both
-    masses.  Rows without an open node or without an entry give loss 0 and gradient 0; a teacher probability on a closed node gives +inf.
+    trajectories.  Entries whose node lies outside [0, V) are absent: -1 is padding.  An entry whose logit is -inf has mass 0, and its node is an
+    entry's all the same, not one of the rest that the tail is spread over.  A node listed twice carries both masses.  Rows without an open node
+    or without an entry above -inf give loss 0 and gradient 0; a teacher probability on a closed node gives +inf.
 
     The gradient reaches `logits` only, in their type, and can be taken once (no double backward); statistics and sums are f32, the sum over
     the rows f64."""

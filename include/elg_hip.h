@@ -489,7 +489,8 @@ int elg_top_logits(const void* z, int64_t z_stride, int type, int64_t R, int64_t
                    int32_t* idx, float* tail, void* stream);
 
 /* Distillation from a teacher's best logits.  top_values (R,k) of top_type at nodes top_idx (R,k) (int32, or int64 with idx_wide);
- * an entry whose node lies outside [0, V) is absent.  q_j = (1 - tail_r) softmax_j(top_values / temperature), p = softmax(z / temperature):
+ * an entry whose node lies outside [0, V) is absent; one of -inf has mass 0, and its node is an entry's all the same.
+ * q_j = (1 - tail_r) softmax_j(top_values / temperature), p = softmax(z / temperature):
  *   L_r = temperature^2 weight_r [ sum_j q_j (log q_j - log p_(i_j)) + tail_r (log tail_r - log sum_(n no entry) p_n) ]
  * tail (R) in [0, 1] or NULL (0), weight (R) or NULL (1).  A row of weight 0 is not read; it, a row without an open node and a row
  * without an entry above -inf have loss 0 and gradient 0.  A teacher probability on a node the student has closed makes the loss +inf.

@@ -115,6 +115,24 @@ def test_distill_any_tail_where_the_entries_are_all_nodes(k):
     assert (got[:-1] == np.inf).all() and np.isfinite(got[-1])
 
 
+@pytest.mark.parametrize("V", [4, 20, 300, 2048, 2049, 9001, 70001])
+def test_distill_entry_without_mass_keeps_its_node_out_of_the_rest(V):
+    """V equal logits, all mass of the entries on node 0, an entry of -inf at node 1, tail 1/2: q_0 = 1/2 on p_0 = 1/V, the tail on the V - 2 nodes
+    of no entry.  Padding with node -1 instead leaves V - 1 of them."""
+    z, tv = torch.zeros(2, V), torch.tensor([[0.0, -np.inf], [0.0, -np.inf]])
+    ti, a = torch.tensor([[0, 1], [0, -1]]).int(), torch.tensor([0.5, 0.5])
+    got, _ = check_losses(z, tv, ti, a)
+    grad = host(lg().distill_loss_grad(z.to(DEV), tv.to(DEV), ti.to(DEV), tail=a.to(DEV), reduction="none")[1])
+    for r, rest in ((0, V - 2), (1, V - 1)):
+        loss = 0.5 * np.log(0.5 * V) + 0.5 * np.log(0.5 * V / rest)
+        assert got[r] == pytest.approx(loss, abs=1e-6)
+        want = np.full(V, 1 / V - 0.5 / rest)
+        want[0] = 1 / V - 0.5
+        if r == 0:
+            want[1] = 1 / V
+        np.testing.assert_allclose(grad[r], want, atol=2e-7)
+
+
 @pytest.mark.parametrize("V", [33, 101, 250, 1001, 2048, 2049, 9001, 70001])
 def test_distill_non_finite_teachers_and_cotangents_reach_what_the_formula_says(V):
     """A NaN or +inf among the teacher's entries is in every q of its row and in no p: the entries' nodes get NaN, the others keep their gradient.
