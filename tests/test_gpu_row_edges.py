@@ -256,3 +256,46 @@ def test_verify_of_more_long_rows_than_one_launch_takes(B, V):
     tile = lambda t: t.repeat(-(-B // n), *[1] * (t.dim() - 1))[:B].to(DEV)  # noqa: E731
     many = lg().verify_draft(P.expand(B, G + 1, V), tile(x), tile(u), draft_probs=Q.expand(B, G, V), lengths=tile(lengths))
     assert torch.equal(many[0], tile(few[0])) and torch.equal(many[1], tile(few[1]))
+
+
+# ------------------------------------------------------------------------------------------------- ranges the documentation names
+@pytest.mark.parametrize("tau", [1e-15, 1e-6, 0.05, 20.0, 1e6, 1e15])
+@pytest.mark.parametrize("V", [17, 101, 300, 1500, 3000, 9001, 70001])
+def test_temperatures_to_both_ends(V, tau):
+    g = rng(V)
+    z = torch.randn(5, V, generator=g) * 4
+    z[1, 1::2] = -np.inf
+    t = z + torch.randn(5, V, generator=g)
+    k = min(V, 33) - 5
+    values, idx, tail = (o.cpu() for o in lg().top_logits(t.to(DEV), k, temperature=tau, with_tail=True))
+    rv, ri = ro.top(host(t), k)
+    ref, err = ro.tail(host(t), ri, tau)
+    np.testing.assert_array_equal(idx.numpy(), ri)
+    # v_exp_f32 gives 0 for what lies below 2^-126: each of up to V - k terms of a sum that is divided by at least 1 can lose that much, and the
+    # bound above allows it once
+    assert (np.abs(host(tail) - ref) <= err + V * 2.0 ** -126).all()
+    check_losses(z, values, idx, tail, tau)
+
+
+def test_rows_beyond_32_bits_of_elements_and_bytes():
+    """22 million rows of 101: 2.2e9 logits.  Row r is row r mod 1000 of a table with a shift of its own: the same order, tail, loss and gradient."""
+    R, V, k, n = 22_000_000, 101, 6, 1000
+    g = rng(1)
+    base = torch.randn(n, V, generator=g).to(DEV)
+    v0, i0, t0 = lg().top_logits(base, k, with_tail=True)
+    z = torch.empty(R, V, dtype=torch.bfloat16, device=DEV)
+    z.view(-1, n, V).copy_(base.bfloat16().expand(R // n, n, V))
+    vb, ib, tb = lg().top_logits(base.bfloat16(), k, with_tail=True)
+    values, idx, tail = lg().top_logits(z, k, with_tail=True)
+    assert all(torch.equal(a.view(-1, *b.shape), b.expand(R // n, *b.shape)) for a, b in ((values, vb), (idx, ib), (tail, tb)))
+    lb, gb = lg().distill_loss_grad(base.bfloat16(), v0, i0, tail=t0, reduction="none")
+    tile = lambda t: t.repeat(R // n, *[1] * (t.dim() - 1))  # noqa: E731
+    loss, grad = lg().distill_loss_grad(z, tile(v0), tile(i0), tail=tile(t0), reduction="none")
+    assert torch.equal(loss.view(-1, n), lb.expand(R // n, n)) and torch.equal(grad.view(-1, n, V), gb.expand(R // n, n, V))
+    # verification of rows behind the 2^31st probability
+    p = torch.softmax(z.view(-1, 2, V)[-4000:].float(), -1)
+    x, u = torch.randint(0, V, (R // 2, 1), device=DEV, dtype=torch.int32), torch.rand(R // 2, 2, device=DEV)
+    z.view(-1, 2, V)[-4000:].copy_(p)
+    tok, acc = lg().verify_draft(z.view(-1, 2, V), x, u)
+    t2, a2 = lg().verify_draft(z.view(-1, 2, V)[-4000:].contiguous(), x[-4000:], u[-4000:])
+    assert torch.equal(tok[-4000:], t2) and torch.equal(acc[-4000:], a2)
