@@ -2,9 +2,9 @@
 verification of drafted choices.  They work on rows as `engine.rollout_forward(..., dump="logits" / "probs")` returns them -- closed nodes
 -inf / 0 -- and on any other rows of 1 to 2^24 entries in f32, bf16 or f16.
 
-    values, idx, tail = top_logits(teacher_logits, 40, with_tail=True)          # once per teacher rollout; 8 bytes per kept logit
-    loss = distill_loss(student_logits, values, idx, tail=tail, temperature=2.0)   # differentiable in the student's logits
-    loss, grad = distill_loss_grad(student_logits, values, idx, tail=tail)      # loss and gradient from one read of the logits
+    values, idx, tail = top_logits(teacher_logits, 40, temperature=2.0, with_tail=True)   # once per teacher rollout; 8 bytes per kept logit
+    loss = distill_loss(student_logits, values, idx, tail=tail, temperature=2.0)          # differentiable in the student's logits
+    loss, grad = distill_loss_grad(student_logits, values, idx, tail=tail, temperature=2.0)   # loss and gradient from one read of the logits
     tokens, accepted = verify_draft(target_probs, drafted, uniforms, draft_probs=draft_probs)
 
 Each is one call into libelg_hip.so (include/elg_hip.h) on the current stream, without a host synchronisation: capturable.  Inputs must
@@ -205,8 +205,8 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_idx: torch.
         q = (1 - tail) softmax(top_values / T),   p = softmax(logits / T)
         L = T^2 weight [ sum_j q_j (log q_j - log p_{i_j})  +  tail (log tail - log p(no entry's node)) ]
 
-    per row; reduction 'none' (...) f32, 'sum', or 'mean' over all rows.  tail (...) f32: the teacher's probability outside its entries
-    (`top_logits(with_tail=True)`), None: the entries hold everything.  weight (...) f32: 0 leaves a row out (it is not read) -- finished
+    per row; reduction 'none' (...) f32, 'sum', or 'mean' over all rows.  tail (...) f32: the teacher's probability outside its entries at
+    the same temperature (`top_logits(with_tail=True)`), None: the entries hold everything.  weight (...) f32: 0 leaves a row out (it is not read) -- finished
     trajectories.  Entries whose node lies outside [0, V) are absent: -1 is padding.  An entry whose logit is -inf has mass 0, and its node is an
     entry's all the same, not one of the rest that the tail is spread over.  A node listed twice carries both masses.  Rows without an open node
     or without an entry above -inf give loss 0 and gradient 0; a teacher probability on a closed node gives +inf.

@@ -161,6 +161,19 @@ def test_distill_non_finite_teachers_and_cotangents_reach_what_the_formula_says(
         assert torch.equal(gx[r], torch.sign(good[1][r]) * sign * np.inf)
 
 
+@pytest.mark.parametrize("V", [101, 1001, 9001])
+@pytest.mark.parametrize("tau", [0.7, 1.0, 2.0])
+def test_distill_of_a_policy_from_itself_is_nothing(V, tau):
+    """With the tail taken at the loss's temperature.  A tail of another temperature belongs to another teacher: a loss above 0."""
+    z = torch.randn(5, V, generator=rng(V)) * 2
+    values, idx, tail = (o.cpu() for o in lg().top_logits(z.to(DEV), 20, temperature=tau, with_tail=True))
+    _, exact = check_losses(z, values, idx, tail, tau)
+    assert np.abs(exact).max() < 1e-10                     # second order in the tail's rounding of 2^-24
+    if tau != 1.0:
+        other = lg().top_logits(z.to(DEV), 20, with_tail=True)[2].cpu()
+        assert (check_losses(z, values, idx, other, tau)[1] > 1e-4).all()
+
+
 @pytest.mark.parametrize("V", [101, 3000])
 def test_distill_backward_reads_what_hooks_on_saved_tensors_give_back(V):
     """A hook that keeps saved tensors on the host: the backward reads the copies it gives back, and the teacher's own memory is free for as long
