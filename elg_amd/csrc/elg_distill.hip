@@ -257,8 +257,8 @@ __device__ __forceinline__ void store_zero(char* grow, const Span<DT>& sp, int t
 }
 
 // One workgroup per row, the row in registers, C chunks a thread (T C 16 bytes of it): one read, one write.  What bounds it is memory as long as
-// two workgroups or more share a CU and their phases overlap (3125 x 32000 f32: 4.5 TB/s); a row of 256 KB takes the CU's registers alone
-// (2048 x 131072 bf16: 286 us, 3.75 TB/s).
+// two workgroups or more share a CU and their phases overlap (3125 x 32000 f32: 4.5 TB/s); the workgroup of a row of 256 KB takes the CU's
+// registers alone (2048 x 131072 bf16: 282 us, 3.8 TB/s).
 template <int DT, int T, int C>
 __global__ __launch_bounds__(T, 4) void distill_row_kernel(const DistillArgs A) {
     static_assert(T >= ELG_TOP_MAX_K, "one entry per thread");
@@ -340,7 +340,7 @@ __global__ __launch_bounds__(T, 4) void distill_row_kernel(const DistillArgs A) 
 
 // Few long rows, or rows beyond what a workgroup can hold: a row is split into segments of SEG_T SEG_C chunks, a workgroup each.  The first
 // kernel leaves every segment's maximum and sum, the second joins them and writes the segments' gradients.
-// 6 rows of 100003 f32: 3.7 and 6.2 us, with nothing but launches and two passes over 2.4 MB in them.
+// 6 rows of 100003 f32: 4 and 6.4 us, with nothing but launches and two passes over 2.4 MB in them.
 constexpr int SEG_T = 256, SEG_C = 4;
 
 template <int DT>
@@ -459,13 +459,15 @@ __global__ __launch_bounds__(SEG_T) void distill_join_kernel(const DistillArgs A
 
 // ---------------------------------------------------------------------------------------------------------------------------------
 // Short rows, G lanes per row (16: four rows to a wave; 64: one).  Lane l holds the nodes n = i G + l, i < NE, and the entries
-// j = e G + l, e < KE, in registers; a row is read and written in runs of G elements, whatever its alignment, and the next row is on its way
-// while this one is worked on (the stores of a row would otherwise stand between it and the next row's loads).
+// j = e G + l, e < KE, in registers; a row is read and written in runs of G elements, whatever its alignment, and up to 16 nodes a lane the
+// next row is on its way while this one is worked on (the stores of a row would otherwise stand between it and the next row's loads).
 // A row of LDS, one float per node, carries what nodes and entries have to tell each other: first the nodes' logits, picked up by the entries,
 // then the entries' teacher masses, picked up by the nodes (-0 marks a node of no entry, and -0 + q = q exactly).  Node n lies at
 // (n % G) PN + n / G there: a lane's own nodes are side by side, so that it moves them 16 bytes at a time, and lanes lie PN apart, so that their
 // banks do not meet.  Waves never wait for each other.
-// 896000 rows of 101 f32 with 40 entries: 243 us, 3.8 TB/s of needed bytes where a copy reaches 4.7; the vector units are busy 73 % of it.
+// The loss of a row takes v_log_f32 and v_rcp_f32, 1 ulp each.  Formed in 64 bits it is no nearer (3.2e-7 off over the rows below either way: the
+// f32 sums and exponentials beneath the logarithms are what is off) and takes 289 us for 246.
+// 896000 rows of 101 f32 with 40 entries: 246 us, 3.75 TB/s of needed bytes where a copy reaches 4.75; the vector units are busy 72 % of it.
 // Instead of one float at a time, aligned 16-byte pieces of whole runs of rows turned through LDS took 358 us, with LDS busy 72 % of it.
 template <int G> __device__ __forceinline__ float gsum(float v) { return G == 16 ? row16_sum(v) : wave_sum(v); }
 template <int G> __device__ __forceinline__ float gmax(float v) { return G == 16 ? row16_max(v) : wave_max(v); }
@@ -733,8 +735,9 @@ struct Plan {
     long long parts;                      // partial losses; 1: the loss itself is written, no scratch for them
     Plan(long long R, long long V, int type) {
         const int vec = type == ELG_F32 ? 4 : 8;
-        // rows that no workgroup can hold, or so few long ones that most of the chip would idle: 6 rows of 100003 f32, the gradient in 35 us and
-        // more by a workgroup each, in 10 us split
+        // rows that no workgroup can hold, or so few long ones that most of the chip would idle.  Loss and gradient, split / by a workgroup each:
+        // 65536 f32, 6 rows 11 / 18 us, 64 rows 18.6 / 21.2, 128 rows 25.7 / 23.7, 256 rows 42 / 32.5; 9001 f32, 6 rows 11.2 / 12.2, 64 rows
+        // 11.6 / 12.2, 192 rows 13.7 / 13.1; 131072 bf16, 64 rows 21.7 / 29, 128 rows 29 / 31, 192 rows 40 / 34
         lanes = V <= 256 ? 16 : V <= 2048 ? 64 : 0;
         split = !lanes && (V > 1024 * 16 * vec || (R <= 64 && V > 1024 * vec));
         segs = split ? (int)((V + vec - 1 + SEG_T * SEG_C * vec - 1) / (SEG_T * SEG_C * vec)) : 0;     // a row may start inside its first 16 bytes
@@ -755,7 +758,9 @@ void launch_row(const DistillArgs& A, int grid, hipStream_t s) {
 }
 
 // Rows of up to 256 logits take a quarter of a wave, up to 2048 a wave (the registers of a lane sized by the next power of two), longer ones a
-// workgroup or several.
+// workgroup or several.  Both sides of the borders, f32, loss and gradient with 30 entries: 15625 rows of 256 in 14.2 us by quarters, 19.5 by
+// waves; 3906 rows of 2048 in 18.9 us by waves, 27.8 by workgroups.  Entry slots a lane, 200000 rows of 101: k = 16 with 1 / 3 / 16 slots 51 / 53 /
+// 108 us, k = 48 with 3 / 16 slots 60 / 112, k = 63 with 16 slots 113; 20000 rows of 1001 by waves, k = 64 with 1 / 4 slots 39.5 / 40.5.
 template <int DT>
 void launch(const DistillArgs& A, const Plan& P, float2* parts, hipStream_t s) {
     const int V = A.V, k = A.k, grid = P.lanes && A.total ? 1 : (int)P.grid;

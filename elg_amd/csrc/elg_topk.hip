@@ -287,9 +287,9 @@ __device__ __noinline__ void top_row_again(const TopArgs& A, long long r, TopSha
 
 // One workgroup per row, the row in registers as order keys, C chunks a thread.  One pass for the threads' maxima, one that gathers the
 // candidates and sums the exponentials of everything below the bound.
-// 512 x 131072 bf16, the best 128: 84 us where its bytes take 28.  A row of 256 KB fills a CU's registers, so each CU works its two rows off one
-// after the other, and between loading them stand the maxima (two 16-bit keys to an operation), the bound's bisection and the ranking, with
-// nothing in flight behind them.  The candidates ranked eight at a time, 112 -> 90 us; keys formed in place of floats, 120 -> 112 us.
+// 512 x 131072 bf16, the best 128: 83 us where its bytes take 28.  One workgroup takes all of a CU's registers, half of them for its row of 256 KB,
+// so each CU works its two rows off one after the other, and between loading them stand the maxima (two 16-bit keys to an operation), the
+// bound's bisection and the ranking, with nothing in flight behind them.  The candidates ranked eight at a time, 112 -> 90 us; keys formed in place of floats, 120 -> 112 us.
 template <int DT, int T, int C>
 __global__ __launch_bounds__(T, 4) void top_row_kernel(const TopArgs A) {
     using W = WordKey<DT>;
@@ -535,7 +535,8 @@ constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_MIRROR4 = 0x1B, DPP_MIRROR8 
 
 // 8 rows to a wave, 4 waves to a workgroup (2 where 4 would need over 64 KB of LDS); waves never wait for each other.  LDS turns the lanes'
 // runs of the order into the rows' packed output.
-// 896000 rows of 101 f32, the best 40 and the tail: 217 us where its bytes take 137 (3.0 TB/s); the sort's exchanges bound it, not memory.
+// 896000 rows of 101 f32, the best 40 and the tail: 219 us where its bytes take 137 (3.0 TB/s; 280 us in the first dozen calls of a process); the
+// sort's exchanges bound it, not memory.
 template <int DT, int NE>
 __global__ __launch_bounds__(256, NE == 32 ? 3 : 4) void top_sort_kernel(const TopArgs A) {
     using K = typename KeyOf<DT>::K;
@@ -614,8 +615,8 @@ void launch_sort(const TopArgs& A, hipStream_t s) {
 // Rows of 257 to 2048 logits: a wave to a row, lane l holding the nodes i 64 + l.  The same selection as a workgroup's, with counts by
 // ballot: a bound from the maxima of groups of NE / 4 nodes, the few candidates above it compacted through LDS, then sorted with one, two or
 // four to a lane.
-// 8000 rows of 1001 f16, the best 63 and the tail: 27 us where its bytes take 4.  All 8000 waves are resident at once, and 1280 vector and 680
-// scalar instructions a row keep the vector units busy two thirds of that time.
+// 8000 rows of 1001 f16, the best 63 and the tail: 27 us where its bytes take 4.  All 8000 waves are resident at once, and 1290 vector and 680
+// scalar instructions a row keep the vector units busy 70 % of the cycles a CU has work.
 template <int NE>
 struct WaveRow {
     unsigned key[NE];
@@ -846,6 +847,8 @@ void launch_wave(const TopArgs& A, hipStream_t s) {
 
 // Up to 256 logits: sorted, eight lanes a row.  Up to 2048: selected, a wave a row.  Longer: a workgroup a row, its size and the chunks a
 // thread holds by what keeps the row in registers (up to 256 KB of them); beyond that the row is read by every pass.
+// Both sides of the borders, f32, the best 30 and the tail: 15625 rows of 256 sorted in 12.7 us, by waves in 23.1; 3906 rows of 2048 by waves in
+// 18.2, by workgroups in 36.0 (bf16: 13.1 / 24.0, 19.6 / 36.4).
 template <int DT>
 void launch_top(const TopArgs& A, hipStream_t s) {
     const bool aligned = !((uintptr_t)A.z & 15) && !(A.stride_bytes & 15);
