@@ -660,7 +660,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistillArgs A)
             const float cot = A.cot && valid ? A.cot[r * A.cot_stride] : 1.f;
             const float Gr = live ? A.scale * cot * x.w * A.tau : 0.f;
             const float c_rest = live ? Gr * (f_rest * inv_S - (a > 0.f && sr > 0.f ? a * inv_sr : 0.f)) : 0.f;
-            const float Gq = Gr * q_scale, c_top = live ? Gr * f_top * inv_S : 0.f;
+            const float Gq = live ? Gr * q_scale : 0.f, c_top = live ? Gr * f_top * inv_S : 0.f;
             if (__any(!live))             // (whatever the nodes of a row without a gradient came to)
 #pragma unroll
                 for (int n = 0; n < NE; ++n) {

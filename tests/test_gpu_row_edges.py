@@ -161,6 +161,24 @@ def test_distill_non_finite_teachers_and_cotangents_reach_what_the_formula_says(
         assert torch.equal(gx[r], torch.sign(good[1][r]) * sign * np.inf)
 
 
+@pytest.mark.parametrize("V", [33, 101, 1001, 2048, 2049, 9001, 70001])
+def test_distill_rows_without_loss_have_none_beside_a_diverged_teacher(V):
+    """Rows of weight 0 and rows whose every node is closed, with NaN in the teacher's logits, in its tail and in the cotangent: 0."""
+    R, k = 9, 5
+    g = rng(V)
+    z = torch.randn(R, V, generator=g)
+    tv, ti = torch.randn(R, k, generator=g), torch.stack([torch.randperm(V, generator=g)[:k] for _ in range(R)]).int()
+    a, w, cot = torch.full((R,), 0.25), torch.ones(R), torch.ones(R)
+    z[[1, 2, 3, 7]] = -np.inf
+    w[[4, 5, 6, 7]] = 0.0
+    tv[[1, 4, 7]], a[[2, 5]], cot[[3, 6]] = float("nan"), float("nan"), float("nan")
+    x = z.to(DEV).requires_grad_(True)
+    loss = lg().distill_loss(x, tv.to(DEV), ti.to(DEV), tail=a.to(DEV), weight=w.to(DEV), reduction="none")
+    (grad,) = torch.autograd.grad(loss, x, cot.to(DEV))
+    assert (loss[1:8] == 0).all() and (grad[1:8] == 0).all()
+    assert torch.isfinite(loss).all() and (loss[[0, 8]] > 0).all() and torch.isfinite(grad).all()
+
+
 @pytest.mark.parametrize("V", [101, 1001, 9001])
 @pytest.mark.parametrize("tau", [0.7, 1.0, 2.0])
 def test_distill_of_a_policy_from_itself_is_nothing(V, tau):
