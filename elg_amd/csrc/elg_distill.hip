@@ -647,7 +647,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistillArgs A)
                 // v_log_f32 takes a subnormal for 0, and a S / sr can be one long before a is: a small mass goes in 2^64 times as large
                 const bool small = a < 1e-18f;
                 const float d_rest = lg2((small ? a * 0x1p64f : a) * S * inv_sr) - (small ? 64.f : 0.f) - (m_rest - m) * A.c2;
-                L += sr <= 0.f ? -ELG_NEG_INF : a * d_rest;        // any mass on a rest that the student has closed
+                L += sr <= 0.f ? -ELG_NEG_INF * S : a * d_rest;    // any mass on a rest that the student has closed (S: 1 or more, or NaN)
             }
             L = live ? L * (LN2 * A.tau * A.tau * x.w) : 0.f;
             if (l == 0 && valid) {

@@ -161,6 +161,19 @@ def test_distill_non_finite_teachers_and_cotangents_reach_what_the_formula_says(
         assert torch.equal(gx[r], torch.sign(good[1][r]) * sign * np.inf)
 
 
+@pytest.mark.parametrize("V", [9, 40, 101, 1001, 2048, 2049, 9001, 70001])
+@pytest.mark.parametrize("odd", [float("nan"), float("inf")])
+def test_distill_nan_is_not_hidden_by_a_closed_rest(V, odd):
+    """The entries hold no mass (tail 1) and the rest is closed: +inf, but NaN where the student's row has diverged."""
+    k = 9
+    z = torch.full((3, V), -np.inf)
+    z[:, :k] = torch.linspace(-1, 1, k)
+    z[1, 4] = odd
+    a = torch.tensor([1.0, 1.0, 0.5])
+    loss, grad = lg().distill_loss_grad(z.to(DEV), torch.zeros(3, k, device=DEV), torch.arange(k, device=DEV).int().expand(3, k), tail=a.to(DEV), reduction="none")
+    assert torch.isnan(loss[1]) and torch.isnan(grad[1]).any() and (loss[[0, 2]] == np.inf).all()
+
+
 @pytest.mark.parametrize("V", [33, 101, 1001, 2048, 2049, 9001, 70001])
 def test_distill_rows_without_loss_have_none_beside_a_diverged_teacher(V):
     """Rows of weight 0 and rows whose every node is closed, with NaN in the teacher's logits, in its tail and in the cotangent: 0."""
