@@ -50,7 +50,10 @@ struct DistillArgs {
     }
 };
 
-// the loss is formed in base 2, like the exponentials, and brought to base e at its end
+// The sum of distances between teacher and student goes 2^-9 times as large (exact), so that 256 distances of the lowest value of f32, which some
+// close their nodes with, add up to a finite number.
+constexpr float SD_SCALE = 0x1p-9f;
+// the logarithms are formed in base 2, like the exponentials, and brought to base e at their end
 constexpr float LN2 = 0.6931471805599453f;
 __device__ __forceinline__ float lg2(float x) { return __builtin_amdgcn_logf(x); }       // v_log_f32
 
@@ -92,7 +95,7 @@ struct RowScalars {
     float q_scale, m, inv_S, c_rest, m_rest, G;
     float a, S, st, sr, sd;
     // mt, mz, mr: largest teacher logit, entry's logit, other logit (-inf: none); st, sz, sr: sums of exponentials relative to each;
-    // sd: sum over entries of e^((t - mt) / tau) ((t - mt) - (z - m))
+    // sd: sum over entries of e^((t - mt) / tau) ((t - mt) - (z - m)), times SD_SCALE
     __device__ __forceinline__ RowScalars(const DistillArgs& A, long long r, float w, float mt, float mz, float mr, float st_, float sz, float sr_, float sd_)
         : st(st_), sr(sr_), sd(sd_) {
         a = A.tail ? A.tail[r] : 0.f;
@@ -126,7 +129,7 @@ __global__ __launch_bounds__(256) void distill_long_loss_kernel(const DistillArg
         double L = 0.0;
         if (u.x != 0.f) {
             const double t = 1.0 / (double)A.tau, d = (double)v.x, S = (double)u.x, st = (double)u.y;
-            if (!(v.x >= 1.f)) L = (1.0 - d) * ((double)u.w / st * t + log((1.0 - d) / st * S));
+            if (!(v.x >= 1.f)) L = (1.0 - d) * ((double)u.w / SD_SCALE / st * t + log((1.0 - d) / st * S));
             if (v.x > 0.f) L += d * (log(d * S / (double)u.z) - (double)v.y * t);
             L *= (double)A.tau * (double)A.tau * (double)v.z;
         }
@@ -323,7 +326,7 @@ __global__ __launch_bounds__(T, 4) void distill_row_kernel(const DistillArgs A) 
         const float tm = mx[0] > ELG_NEG_INF ? mx[0] : 0.f, zm = mx[1] > ELG_NEG_INF ? mx[1] : 0.f, m = fmaxf(mx[1], mx[2]);
         const float mine = en.i >= 0 ? ex2((en.t - tm) * A.c2) : 0.f;
         float sm[4] = {mine, first ? ex2((en.z - zm) * A.c2) : 0.f, rest.to(mx[2], A.c2),
-                       mine > 0.f || mine != mine ? mine * ((en.t - tm) - (en.z - m)) : 0.f};
+                       mine > 0.f || mine != mine ? mine * (SD_SCALE * ((en.t - tm) - (en.z - m))) : 0.f};
         if (tid < k) ee[tid] = mine;
         if (en.i >= 0) bits[(en.i + sp.shift) >> 5] = 0u;              // clean for the next row
         bsum.template run<false>(sm);
@@ -443,7 +446,7 @@ __global__ __launch_bounds__(SEG_T) void distill_join_kernel(const DistillArgs A
     const float tm = mx[0] > ELG_NEG_INF ? mx[0] : 0.f, zm = mx[1] > ELG_NEG_INF ? mx[1] : 0.f, m = fmaxf(mx[1], mx[2]);
     const float mine = en.i >= 0 ? ex2((en.t - tm) * A.c2) : 0.f;
     float sm[4] = {mine, first ? ex2((en.z - zm) * A.c2) : 0.f, rest.to(mx[2], A.c2),
-                   mine > 0.f || mine != mine ? mine * ((en.t - tm) - (en.z - m)) : 0.f};
+                   mine > 0.f || mine != mine ? mine * (SD_SCALE * ((en.t - tm) - (en.z - m))) : 0.f};
     if (tid < k) ee[tid] = mine;
     bsum.template run<false>(sm);
     const RowScalars s(A, r, w, mx[0], mx[1], mx[2], sm[0], sm[1], sm[2], sm[3]);
@@ -630,7 +633,7 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistillArgs A)
             sr += rest ? x.z[n] : 0.f;
         }
 #pragma unroll
-        for (int e = 0; e < KE; ++e) sd += q[e] > 0.f || q[e] != q[e] ? q[e] * ((x.t[e] - tm) - (zi[e] - m)) : 0.f;
+        for (int e = 0; e < KE; ++e) sd += q[e] > 0.f || q[e] != q[e] ? q[e] * (SD_SCALE * ((x.t[e] - tm) - (zi[e] - m))) : 0.f;
         st = gsum<G>(st);
         sz = gsum<G>(sz);
         sr = gsum<G>(sr);
@@ -641,15 +644,21 @@ __global__ __launch_bounds__(256) void distill_small_kernel(const DistillArgs A)
         const bool live = x.w != 0.f && !(S <= 0.f) && !(st <= 0.f);
         if (A.loss_rows || A.part || A.total) {
             const float d = gsum<G>(sd);
-            float L = 0.f;
-            if (!(a >= 1.f)) L = (d * q_scale) * A.c2 + (1.f - a) * lg2(q_scale * S);
+            // The distances times tau^2 c2 ln 2 = tau, apart from the logarithms: a distance of the type's lowest value times c2 would be infinite.
+            // All of it SD_SCALE times as large until it has met its weight.
+            float L = 0.f, lg = 0.f;
+            if (!(a >= 1.f)) {
+                L = (d * q_scale) * A.tau;
+                lg = (1.f - a) * lg2(q_scale * S);
+            }
             if (a > 0.f) {
                 // v_log_f32 takes a subnormal for 0, and a S / sr can be one long before a is: a small mass goes in 2^64 times as large
                 const bool small = a < 1e-18f;
-                const float d_rest = lg2((small ? a * 0x1p64f : a) * S * inv_sr) - (small ? 64.f : 0.f) - (m_rest - m) * A.c2;
-                L += sr <= 0.f ? -ELG_NEG_INF * S : a * d_rest;    // any mass on a rest that the student has closed (S: 1 or more, or NaN)
+                lg += a * (lg2((small ? a * 0x1p64f : a) * S * inv_sr) - (small ? 64.f : 0.f));
+                L -= (SD_SCALE * a * A.tau) * (m_rest - m);
+                if (sr <= 0.f) lg = -ELG_NEG_INF * S;              // any mass on a rest that the student has closed (S: 1 or more, or NaN)
             }
-            L = live ? L * (LN2 * A.tau * A.tau * x.w) : 0.f;
+            L = live ? (L + lg * (SD_SCALE * LN2 * A.tau * A.tau)) * x.w * (1.f / SD_SCALE) : 0.f;
             if (l == 0 && valid) {
                 if (A.loss_rows) A.loss_rows[r] = L * A.scale;
                 lacc += (double)L;

@@ -161,6 +161,29 @@ def test_distill_non_finite_teachers_and_cotangents_reach_what_the_formula_says(
         assert torch.equal(gx[r], torch.sign(good[1][r]) * sign * np.inf)
 
 
+@pytest.mark.parametrize("V", [12, 101, 1001, 2048, 2049, 9001, 70001])
+@pytest.mark.parametrize("tau", [1e-3, 0.1, 1.0, 3.0])
+def test_distill_mass_on_nodes_closed_by_the_lowest_value(V, tau):
+    """A student that closes nodes by the lowest value of f32 instead of -inf, a teacher that does not: the loss is large and finite wherever f32
+    holds it, T (mass there) 3.4e38, whether one entry lies there, most of them, or the rest."""
+    low, k = torch.finfo(torch.float32).min, 6
+    z = torch.linspace(-2, 2, V).expand(5, V).clone()
+    z[0, 2] = low
+    z[1, :4] = low
+    z[2, k:] = low
+    z[3, 1:] = low
+    z[4] = low                                             # all alike: an ordinary row
+    a = torch.tensor([0.0, 0.25, 0.25, 0.25, 0.25])
+    w = torch.tensor([0.3, 0.3, 0.3, -0.3, 1.0])
+    d = [t.to(DEV) for t in (z, torch.zeros(5, k), torch.arange(k).int().expand(5, k), a, w)]
+    more = dict(tail=d[3], temperature=tau, weight=d[4])
+    got = host(lg().distill_loss(d[0], d[1], d[2], reduction="none", **more))
+    # log p there is (low - m) / T to 37 digits; a sum of six terms and a dozen products, each rounded by 2^-24
+    want = -low * tau * w[:4].double().numpy() * np.array([1 / 6, 0.75 * 4 / 6, 0.25, 0.75 * 5 / 6 + 0.25])
+    assert np.isfinite(got).all() and (np.abs(got[:4] - want) <= 20 * ro.U * np.abs(want)).all(), (got, want)
+    assert abs(got[4]) < 20 * tau * tau and lg().distill_loss(d[0], d[1], d[2], **more).item() == pytest.approx(want.sum() / 5, rel=1e-5)
+
+
 @pytest.mark.parametrize("V", [9, 40, 101, 1001, 2048, 2049, 9001, 70001])
 @pytest.mark.parametrize("odd", [float("nan"), float("inf")])
 def test_distill_nan_is_not_hidden_by_a_closed_rest(V, odd):
