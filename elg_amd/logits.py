@@ -160,7 +160,7 @@ class _DistillLoss(torch.autograd.Function):
     def forward(ctx, logits, teacher, reduction, values, idx, tail, weight):
         z = _rows(logits, "logits")
         scale = _scale(reduction, z.shape[0])
-        ctx.type, ctx.temperature, ctx.scale, ctx.reduction, ctx.shape = teacher.type, teacher.temperature, scale, reduction, values.shape
+        ctx.dtype, ctx.temperature, ctx.scale, ctx.reduction, ctx.shape = logits.dtype, teacher.temperature, scale, reduction, values.shape
         # the teacher's tensors too, and nothing beside: writing to one before the backward is an error, not a wrong gradient, hooks on saved
         # tensors see what the backward reads, and it is all freed with the graph
         ctx.save_for_backward(logits, values, idx, tail, weight)
@@ -176,9 +176,15 @@ class _DistillLoss(torch.autograd.Function):
     @staticmethod
     def gradient(ctx, gout):
         logits, values, idx, tail, weight = ctx.saved_tensors
-        if values.shape != ctx.shape or idx.shape != ctx.shape or (tail is not None and tail.shape != ctx.shape[:-1]) \
-                or (weight is not None and weight.shape != ctx.shape[:-1]):
-            raise RuntimeError("elg_amd: a hook on saved tensors gave back a teacher of another shape than was saved")
+        # what a hook gives back goes to the kernel by its address: it has to be what was saved
+        dev, lead = gout.get_device(), ctx.shape[:-1]
+        if logits.shape[:-1] != lead or logits.get_device() != dev or logits.dtype is not ctx.dtype or values.shape != ctx.shape \
+                or values.get_device() != dev or values.dtype not in _TYPES or idx.shape != ctx.shape or idx.get_device() != dev \
+                or (idx.dtype is not torch.int32 and idx.dtype is not torch.int64):
+            raise RuntimeError("elg_amd: a hook on saved tensors gave back other logits or another teacher than were saved")
+        for t in (tail, weight):
+            if t is not None and (t.shape != lead or t.get_device() != dev or t.dtype is not torch.float32):
+                raise RuntimeError("elg_amd: a hook on saved tensors gave back another tail or weight than was saved")
         z = _rows(logits, "logits")
         grad = z.new_empty(logits.shape)
         if z.shape[0]:
@@ -186,7 +192,7 @@ class _DistillLoss(torch.autograd.Function):
                 gout = gout.float().contiguous()
             teacher = (values.contiguous(), idx.contiguous(), None if tail is None else tail.contiguous(),
                        None if weight is None else weight.contiguous())
-            _distill_call(z, ctx.type, teacher, ctx.temperature, cot=gout, cot_stride=int(ctx.reduction == "none"), scale=ctx.scale, grad=grad)
+            _distill_call(z, _TYPES[z.dtype], teacher, ctx.temperature, cot=gout, cot_stride=int(ctx.reduction == "none"), scale=ctx.scale, grad=grad)
         return grad, None, None, None, None, None, None
 
     @staticmethod

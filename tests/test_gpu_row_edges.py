@@ -260,6 +260,20 @@ def test_distill_backward_reads_what_hooks_on_saved_tensors_give_back(V):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("which", ["logits", "values", "idx", "tail", "weight"])
+@pytest.mark.parametrize("how", [lambda t: t.cpu(), lambda t: t[:-1], lambda t: t.double()], ids=["host", "shape", "type"])
+def test_distill_refuses_what_else_a_hook_gives_back(which, how):
+    R, V, k = 4, 60, 3
+    tensors = dict(logits=torch.randn(R, V, device=DEV, requires_grad=True), values=torch.randn(R, k, device=DEV), tail=torch.rand(R, device=DEV),
+                   idx=torch.zeros(R, k, device=DEV, dtype=torch.int32), weight=torch.rand(R, device=DEV) + 1)
+    place = list(("logits", "values", "idx", "tail", "weight")).index(which)
+    packed = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (packed.append(t), len(packed) - 1)[1], lambda i: how(packed[i].detach()) if i == place else packed[i]):
+        loss = lg().distill_loss(tensors["logits"], tensors["values"], tensors["idx"], tail=tensors["tail"], weight=tensors["weight"])
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(loss, tensors["logits"])
+
+
 def test_distill_teacher_is_freed_with_the_graph():
     import weakref
     z, ti = torch.randn(4, 50, device=DEV, requires_grad=True), torch.zeros(4, 3, device=DEV, dtype=torch.int32)
