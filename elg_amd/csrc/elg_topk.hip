@@ -289,7 +289,8 @@ __device__ __noinline__ void top_row_again(const TopArgs& A, long long r, TopSha
 // candidates and sums the exponentials of everything below the bound.
 // 512 x 131072 bf16, the best 128: 83 us where its bytes take 28.  One workgroup takes all of a CU's registers, half of them for its row of 256 KB,
 // so each CU works its two rows off one after the other, and between loading them stand the maxima (two 16-bit keys to an operation), the
-// bound's bisection and the ranking, with nothing in flight behind them.  The candidates ranked eight at a time, 112 -> 90 us; keys formed in place of floats, 120 -> 112 us.
+// bound's bisection and the ranking, with nothing in flight behind them.  The candidates ranked eight at a time, 112 -> 90 us; keys formed in
+// place of floats, 120 -> 112 us.
 template <int DT, int T, int C>
 __global__ __launch_bounds__(T, 4) void top_row_kernel(const TopArgs A) {
     using W = WordKey<DT>;
